@@ -234,6 +234,92 @@ int mi_rmsnorm_matmul_bf16(const void* x, const void* gamma, const void* W, void
 int mi_matmul_lhsT_rhs_bf16_noalloc(const void* lhsT, const void* rhs, void* out, int M, int N, int K,
                                     const mi_tile_cfg* cfg, void* stream);
 
+/* ---- The operators of a transformer block's training step ---------------
+ * No counterpart in the reference, which has products and the fused norm
+ * only.  Each takes one argument structure; a call that needs device memory
+ * of its own takes it from the caller (workspace, 16-byte aligned, as many
+ * bytes as the operator's _workspace call says for the same arguments), so
+ * no call allocates and any may be captured in a HIP graph.  Workspaces hold
+ * nothing between calls.  No output may overlap an input, another output or
+ * the workspace (MI_E_ARGS); pointers have their element's alignment, and
+ * where rows start on 16 bytes the kernels use it. */
+enum { MI_DTYPE_BF16 = 0, MI_DTYPE_F16 = 1, MI_DTYPE_F32 = 2 };
+
+/* y[r,d] = (x[r,d] - mean_r) * rstd_r * weight[d] + bias[d], with mean_r =
+ * sum_d x / D, rstd_r = 1 / sqrt(sum_d (x - mean_r)^2 / D + eps); statistics
+ * in fp32, one rounding to y's type (x's).  Rows of x are ldx elements apart
+ * (0: every row the same), y is contiguous.  weight, bias [D]: of x's type,
+ * or fp32 (params_f32); NULL for 1 and 0.  mean, rstd [rows] fp32: what the
+ * gradient takes; NULL where not wanted.  rows may be 0; any D > 0. */
+typedef struct {
+  const void *x, *weight, *bias;
+  void* y;
+  float *mean, *rstd;
+  long long rows, ldx;
+  int D, dtype, params_f32;
+  float eps;
+} mi_layer_norm_args;
+int mi_layer_norm(const mi_layer_norm_args* args, void* stream);
+
+/* The gradients of mi_layer_norm.  With xh = (x - mean) * rstd and g = dout
+ * * weight: dx = rstd * (g - mean_d(g) - xh * mean_d(g * xh)) of x's type,
+ * contiguous; dweight = sum_r dout * xh and dbias = sum_r dout of the
+ * parameters' type (params_f32).  Each output NULL where not wanted.  Column
+ * sums are fp32 in an order fixed by the sizes; rows == 0 leaves them 0. */
+typedef struct {
+  const void *dout, *x, *weight;
+  const float *mean, *rstd;
+  void *dx, *dweight, *dbias;
+  long long rows, lddout, ldx;
+  int D, dtype, params_f32;
+} mi_layer_norm_grad_args;
+int mi_layer_norm_backward_workspace(const mi_layer_norm_grad_args* args, unsigned long long* bytes);
+int mi_layer_norm_backward(const mi_layer_norm_grad_args* args, void* workspace, unsigned long long workspace_bytes,
+                           void* stream);
+
+/* out = act(lhs . rhs + bias) + residual, bf16 operands and outputs, fp32
+ * accumulation over the whole K, one rounding.  lhs [M,K]; rhs [K,N], or
+ * [N,K] with rhs_transposed (out = act(lhs . rhs^T + bias) + residual); bias
+ * [N] bf16, or fp32 (bias_f32); residual, out, pre [M,N]; all contiguous.
+ * bias, residual: NULL for none.  pre: NULL, or gets lhs . rhs + bias, which
+ * the gradient takes.  Any M, N, K >= 0 (K = 0: a product of 0); operands
+ * under 4 GiB (MI_E_RANGE).  Operands whose rows do not start on 16 bytes
+ * (K or, untransposed, N no multiple of 8) are copied to padded rows in the
+ * workspace first.
+ *
+ * cfg: block_m, block_n, block_k, waves, lds_stages and variant (1: rhs read
+ * non-temporally, for few rows) of one of mi_epilogue_config's, split_k
+ * 1..16 (every part at least one K tile) and group_m (0: 8); NULL: the
+ * library's choice for the shape. */
+enum { MI_ACT_NONE = 0, MI_ACT_RELU = 1, MI_ACT_GELU = 2, MI_ACT_GELU_TANH = 3, MI_ACT_SILU = 4 };
+typedef struct {
+  const void *lhs, *rhs, *bias, *residual;
+  void *out, *pre;
+  int M, N, K, rhs_transposed, activation, bias_f32;
+} mi_epilogue_args;
+int mi_epilogue_num_configs(void);
+int mi_epilogue_config(int idx, mi_tile_cfg* cfg);
+int mi_epilogue_default_config(int M, int N, int K, int rhs_transposed, mi_tile_cfg* cfg);
+int mi_matmul_epilogue_workspace(const mi_epilogue_args* args, const mi_tile_cfg* cfg, unsigned long long* bytes);
+int mi_matmul_epilogue_bf16(const mi_epilogue_args* args, const mi_tile_cfg* cfg, void* workspace,
+                            unsigned long long workspace_bytes, void* stream);
+
+/* The gradients of mi_matmul_epilogue_bf16.  dpre = dout * act'(pre), in
+ * fp32; dlhs = dpre . rhs^T and drhs = lhs^T . dpre (of rhs's layout) take it
+ * rounded to bf16, the type of the matrix cores' operands; dbias = sum_m dpre
+ * takes it unrounded and has the bias's type.  The residual's gradient is
+ * dout itself.  pre: what the forward call wrote (NULL for MI_ACT_NONE).
+ * Each output NULL where not wanted.  drhs's product may take split-K
+ * workspace as mi_matmul_lhsT_rhs_bf16 does. */
+typedef struct {
+  const void *dout, *lhs, *rhs, *pre;
+  void *dlhs, *drhs, *dbias;
+  int M, N, K, rhs_transposed, activation, bias_f32;
+} mi_epilogue_grad_args;
+int mi_matmul_epilogue_backward_workspace(const mi_epilogue_grad_args* args, unsigned long long* bytes);
+int mi_matmul_epilogue_backward_bf16(const mi_epilogue_grad_args* args, void* workspace,
+                                     unsigned long long workspace_bytes, void* stream);
+
 /* Device discovery: number of visible HIP devices and the gfx arch name of
  * device 0 (written to arch, at most arch_len bytes).  Returns 0 or -error.
  * Replaces detect_neuron_cores()

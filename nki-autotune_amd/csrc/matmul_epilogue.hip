@@ -1,0 +1,520 @@
+// matmul_epilogue.hip -- mi_matmul_epilogue_bf16 and its gradient: argument
+// checks, the config a call takes, workspaces and launches (products:
+// mi_mm_epi.hpp).
+#include "mi_capi_internal.hpp"
+#include "mi_epi_table.hpp"
+#include "mi_norm.hpp"
+
+namespace {
+
+using mi::EpiEntry;
+using mi::EpiMM;
+using mi::EpiOut;
+using mi::capi::fail;
+using mi::capi::kMaxOffset;
+using mi::capi::kMaxSplit;
+
+// ---- kernels beside the products --------------------------------------
+
+// dst[r][0, cp) = src[r][0, c), then zeros: rows that start on 16 bytes.
+__global__ __launch_bounds__(256) void pad_rows_kernel(const uint16_t* __restrict__ src, uint16_t* __restrict__ dst,
+                                                       long long rows, int c, int cp) {
+  const int groups = cp / 8;
+  const long long n = rows * groups;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+    const long long r = i / groups;
+    const int d = (int)(i - r * groups) * 8;
+    const uint16_t* s = src + (size_t)r * (size_t)c;
+    uint32_t v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = d + k < c ? s[d + k] : 0u;
+    *(mi::u32x4_t*)(dst + (size_t)r * (size_t)cp + d) =
+        mi::u32x4_t{v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16};
+  }
+}
+
+// dst[r][0, c) = src[r][0, c) of rows cp apart (dst rows c apart): the way back.
+__global__ __launch_bounds__(256) void unpad_rows_kernel(const uint16_t* __restrict__ src, uint16_t* __restrict__ dst,
+                                                         long long rows, int c, int cp) {
+  const long long n = rows * c;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+    const long long r = i / c;
+    dst[i] = src[(size_t)r * (size_t)cp + (size_t)(i - r * c)];
+  }
+}
+
+// out = act(sum over parts of ws[part][M][ldw] + bias) + residual, parts in
+// order (parts == 0: a product of 0); 8 columns of one row a thread.
+__global__ __launch_bounds__(256) void epi_sum_kernel(const float* __restrict__ ws, int parts, int ldw, EpiOut e) {
+  const int groups = ldw / 8;
+  const long long n = (long long)e.M * groups;
+  const size_t stride = (size_t)e.M * (size_t)ldw;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+    const int m = (int)(i / groups), c = (int)(i - (long long)m * groups) * 8;
+    e.columns(c);
+    e.fetch(0, m, c);
+    float v[8] = {};
+    if (parts > 0) {
+      const float* at = ws + (size_t)m * (size_t)ldw + c;
+      const mi::f32x4_t lo = mi::sum_in_order<0>((const mi::f32x4_t*)at, stride, parts);
+      const mi::f32x4_t hi = mi::sum_in_order<0>((const mi::f32x4_t*)(at + 4), stride, parts);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        v[k] = lo[k];
+        v[4 + k] = hi[k];
+      }
+    }
+    e.apply(0, m, c, v);
+  }
+}
+
+// dpre[m][0, np) = bf16(dout * act'(pre)) with zeros past N, and the column
+// sums of the unrounded values over this block's rows: blockIdx.x takes 512
+// columns, the block's 4 waves rows 4 * blockIdx.y + wave, + 4 * gridDim.y, ...
+struct ActGrad {
+  const uint16_t *dout, *pre;
+  uint16_t* dpre;  // NULL: not wanted
+  float* part;     // [gridDim.y][N], NULL: not wanted
+  int M, N, np, act;
+  bool vec;
+};
+__global__ __launch_bounds__(256) void act_grad_kernel(const ActGrad p) {
+  __shared__ float xs[4][512 + 8];
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+  const int c = (int)blockIdx.x * 512 + lane * 8;
+  float sum[8] = {};
+  const int step = 4 * (int)gridDim.y;
+  auto load = [&](const uint16_t* q, int m, float (&v)[8]) __attribute__((always_inline)) {
+    const uint16_t* at = q + (size_t)m * (size_t)p.N + c;
+    if (p.vec) {
+      mi::unpack8(*(const mi::u32x4_t*)at, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = c + i < p.N ? mi::bf16lo((uint32_t)at[i]) : 0.0f;
+    }
+  };
+  constexpr int U = 4;
+  if (c < p.np)
+    for (int m0 = 4 * (int)blockIdx.y + wave; m0 < p.M; m0 += U * step) {
+      float d[U][8], x[U][8];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int m = m0 + u * step;
+        if (m >= p.M) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) d[u][i] = x[u][i] = 0.0f;
+          continue;
+        }
+        load(p.dout, m, d[u]);
+        if (p.pre) load(p.pre, m, x[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (p.pre)
+          mi::with_act(p.act, [&](auto a_c) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) d[u][i] *= mi::act_slope<decltype(a_c)::value>(x[u][i]);
+          });
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum[i] += d[u][i];
+        const int m = m0 + u * step;
+        if (p.dpre && m < p.M) *(mi::u32x4_t*)(p.dpre + (size_t)m * (size_t)p.np + c) = mi::pack8(d[u]);
+      }
+    }
+  if (!p.part) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) xs[wave][lane * 8 + i] = sum[i];
+  __syncthreads();
+  for (int k = (int)threadIdx.x; k < 512; k += 256) {
+    const int n = (int)blockIdx.x * 512 + k;
+    if (n < p.N) p.part[(size_t)blockIdx.y * (size_t)p.N + n] = ((xs[0][k] + xs[1][k]) + xs[2][k]) + xs[3][k];
+  }
+}
+
+// ---- host ----------------------------------------------------------------
+
+int launched(const char* what) {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? MI_OK : fail(-(int)e, "%s: %s", what, hipGetErrorString(e));
+}
+
+unsigned blocks_for(long long items) {
+  const long long b = (items + 255) / 256;
+  return (unsigned)(b < 1 ? 1 : b > 8192 ? 8192 : b);
+}
+
+int up8(int v) { return (v + 7) / 8 * 8; }
+size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+bool at16(const void* p) { return (uintptr_t)p % 16 == 0; }
+
+bool overlap(const void* p, size_t pb, const void* q, size_t qb) {
+  return p && q && pb && qb && (uintptr_t)p < (uintptr_t)q + qb && (uintptr_t)q < (uintptr_t)p + pb;
+}
+struct Range {
+  const void* p;
+  size_t n;
+};
+// No output shares a byte with an input or another output.
+template <size_t NO, size_t NI>
+int check_overlap(const Range (&out)[NO], const Range (&in)[NI]) {
+  for (size_t i = 0; i < NO; ++i) {
+    for (const Range& q : in)
+      if (overlap(out[i].p, out[i].n, q.p, q.n)) return fail(MI_E_ARGS, "an output overlaps an input");
+    for (size_t j = 0; j < i; ++j)
+      if (overlap(out[i].p, out[i].n, out[j].p, out[j].n)) return fail(MI_E_ARGS, "two outputs overlap");
+  }
+  return MI_OK;
+}
+
+const EpiEntry* table(bool bt, int* n) { return bt ? mi::epi_table_nt(n) : mi::epi_table_nn(n); }
+
+const EpiEntry* find(bool bt, const mi_tile_cfg& c) {
+  int n = 0;
+  const EpiEntry* t = table(bt, &n);
+  for (int i = 0; i < n; ++i) {
+    const mi_tile_cfg& x = t[i].cfg;
+    if (x.block_m == c.block_m && x.block_n == c.block_n && x.block_k == c.block_k && x.waves == c.waves &&
+        x.lds_stages == c.lds_stages && x.variant == c.variant)
+      return &t[i];
+  }
+  return nullptr;
+}
+
+// The library's choice of a config for a product of these sizes.
+mi_tile_cfg pick(int M, int N, int K, bool bt) {
+  (void)bt;
+  mi_tile_cfg c = {256, 256, 64, 8, 2, 1, 8, 0};
+  const auto tiles = [&](int bm, int bn) { return (long long)((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
+  if (M <= 64) c = {M <= 32 ? 32 : 64, 128, 64, 4, 4, 1, 8, 1};
+  else if (tiles(256, 256) < 200) c = tiles(128, 128) >= 200 ? mi_tile_cfg{128, 128, 64, 4, 2, 1, 8, 0} : mi_tile_cfg{64, 64, 64, 4, 4, 1, 8, 0};
+  const long long t = tiles(c.block_m, c.block_n);
+  const int kt = (K + 63) / 64;
+  int parts = 1;
+  while (parts < kMaxSplit && t * parts * 2 <= 512 && kt / (parts * 2) >= 8) parts *= 2;
+  const int each = (kt + parts - 1) / parts;
+  c.split_k = each > 0 ? (kt + each - 1) / each : 1;
+  return c;
+}
+
+// One product A . B or A . B^T with an epilogue, operands already in rows of
+// 16 bytes.
+struct Product {
+  EpiMM mm;
+  const EpiEntry* e;
+  int ldw;
+  size_t ws_bytes;
+};
+int plan(const uint16_t* a, int lda, const uint16_t* b, int ldb, long long b_rows, int M, int N, int K, bool bt,
+         const mi_tile_cfg* cfg, Product* out) {
+  mi_tile_cfg c = cfg ? *cfg : pick(M, N, K, bt);
+  if (c.split_k < 1 || c.split_k > kMaxSplit) return fail(MI_E_SPLIT, "split_k=%d outside [1, %d]", c.split_k, kMaxSplit);
+  if (c.group_m < 0) return fail(MI_E_ARGS, "group_m=%d negative", c.group_m);
+  const EpiEntry* e = find(bt, c);
+  if (!e)
+    return fail(MI_E_NO_INSTANCE, "no compiled instance for the epilogue product with bm=%d bn=%d bk=%d waves=%d stages=%d variant=%d",
+                c.block_m, c.block_n, c.block_k, c.waves, c.lds_stages, c.variant);
+  const long long kt = ((long long)K + c.block_k - 1) / c.block_k, each = (kt + c.split_k - 1) / c.split_k;
+  if ((long long)(c.split_k - 1) * each >= kt && c.split_k > 1)
+    return fail(MI_E_SPLIT, "split_k=%d leaves a K part empty at K=%d, block_k=%d", c.split_k, K, c.block_k);
+  // Loads run up to a block past the last row and a K tile past the last column.
+  const unsigned long long a_span = ((unsigned long long)M + c.block_m) * lda * 2ull + 16ull * c.block_k;
+  const unsigned long long b_span = bt ? ((unsigned long long)N + c.block_n) * ldb * 2ull + 16ull * c.block_k
+                                       : ((unsigned long long)K + c.block_k) * ldb * 2ull + 2ull * c.block_n;
+  if (a_span > kMaxOffset || b_span > kMaxOffset)
+    return fail(MI_E_RANGE, "operand spans exceed 32-bit buffer offsets (%llu, %llu bytes)", a_span, b_span);
+  out->e = e;
+  out->ldw = up8(N);
+  out->ws_bytes = c.split_k > 1 ? (size_t)c.split_k * (size_t)M * (size_t)out->ldw * 4 : 0;
+  if (out->ws_bytes > mi::capi::kMaxWorkspace)
+    return fail(MI_E_RANGE, "split-K workspace of %zu bytes exceeds %llu", out->ws_bytes, mi::capi::kMaxWorkspace);
+  out->mm = EpiMM{a, b, (uint32_t)((size_t)M * lda * 2), (uint32_t)((size_t)b_rows * ldb * 2), M, N, K, lda, ldb,
+                  c.group_m > 0 ? c.group_m : 8, c.split_k, 0, 0, 0, 0};
+  return MI_OK;
+}
+int run(const Product& p, const EpiOut& o, float* ws, hipStream_t s) {
+  if (p.mm.parts > 1) {
+    p.e->split(p.mm, ws, p.ldw, s);
+    const int rc = launched("epilogue product");
+    if (rc != MI_OK) return rc;
+    epi_sum_kernel<<<dim3(blocks_for((long long)o.M * (p.ldw / 8))), dim3(256), 0, s>>>(ws, p.mm.parts, p.ldw, o);
+    return launched("sum of the parts");
+  }
+  p.e->direct(p.mm, o, s);
+  return launched("epilogue product");
+}
+
+// An operand that needs padded rows: its copy's place in the workspace.
+struct Padded {
+  bool on;
+  int ld;
+  size_t at, bytes;
+};
+Padded padded(const void* p, long long rows, int c, size_t* ws) {
+  Padded q = {c % 8 != 0 || !at16(p), up8(c), 0, 0};
+  if (q.on) {
+    q.at = *ws;
+    q.bytes = (size_t)rows * (size_t)q.ld * 2;
+    *ws += up256(q.bytes);
+  }
+  return q;
+}
+int pad(const void* src, char* ws, const Padded& q, long long rows, int c, hipStream_t s) {
+  if (!q.on) return MI_OK;
+  pad_rows_kernel<<<dim3(blocks_for(rows * (q.ld / 8))), dim3(256), 0, s>>>((const uint16_t*)src, (uint16_t*)(ws + q.at),
+                                                                           rows, c, q.ld);
+  return launched("padded copy");
+}
+const uint16_t* placed(const void* src, char* ws, const Padded& q) {
+  return (const uint16_t*)(q.on ? ws + q.at : src);
+}
+
+int check_sizes(int M, int N, int K, int act) {
+  if (M < 0 || N < 0 || K < 0) return fail(MI_E_ARGS, "negative size M=%d N=%d K=%d", M, N, K);
+  if (act < MI_ACT_NONE || act > MI_ACT_SILU) return fail(MI_E_ARGS, "unknown activation %d", act);
+  const unsigned long long lim = kMaxOffset / 2;
+  if ((unsigned long long)M * K > lim || (unsigned long long)K * N > lim || (unsigned long long)M * N > 1ull << 40)
+    return fail(MI_E_RANGE, "operand spans exceed 32-bit buffer offsets (M=%d N=%d K=%d)", M, N, K);
+  return MI_OK;
+}
+
+// Everything that a forward call decides before it launches.
+struct Fwd {
+  Padded lhs, rhs;
+  Product mm;
+  size_t part_at, bytes;
+};
+int fwd_plan(const mi_epilogue_args* a, const mi_tile_cfg* cfg, char* ws, Fwd* f) {
+  const int rc = check_sizes(a->M, a->N, a->K, a->activation);
+  if (rc != MI_OK) return rc;
+  *f = Fwd{};
+  if (a->M == 0 || a->N == 0 || a->K == 0) return MI_OK;
+  const bool bt = a->rhs_transposed != 0;
+  const int b_rows = bt ? a->N : a->K, b_cols = bt ? a->K : a->N;
+  f->lhs = padded(a->lhs, a->M, a->K, &f->bytes);
+  f->rhs = padded(a->rhs, b_rows, b_cols, &f->bytes);
+  f->part_at = f->bytes;
+  const int prc = plan(placed(a->lhs, ws, f->lhs), f->lhs.ld, placed(a->rhs, ws, f->rhs), f->rhs.ld, b_rows, a->M, a->N,
+                       f->lhs.ld, bt, cfg, &f->mm);
+  f->bytes += f->mm.ws_bytes;
+  return prc;
+}
+
+struct Bwd {
+  Padded dout, lhs, rhs;      // dout: dpre's place, or dout's padded copy
+  bool dpre;                  // dout * act'(pre) goes to that place
+  Product dlhs;
+  size_t part_at, drhs_at, bias_at, bytes;
+  int chunks, kp;
+  bool drhs_padded;
+};
+int bwd_plan(const mi_epilogue_grad_args* a, char* ws, Bwd* b) {
+  const int rc = check_sizes(a->M, a->N, a->K, a->activation);
+  if (rc != MI_OK) return rc;
+  *b = Bwd{};
+  if (a->M == 0 || a->N == 0) return MI_OK;
+  const bool bt = a->rhs_transposed != 0;
+  const long long M = a->M;
+  b->kp = up8(a->K);
+  if (a->dbias) {
+    const int xb = (up8(a->N) + 511) / 512;
+    const int rows4 = (a->M + 3) / 4, want = 2048 / xb;
+    b->chunks = want < 1 ? 1 : want > 256 ? 256 : want;
+    if (b->chunks > rows4) b->chunks = rows4;
+    b->bias_at = b->bytes;
+    b->bytes += up256((size_t)b->chunks * a->N * 4);
+  }
+  if (a->K == 0 || (!a->dlhs && !a->drhs)) return MI_OK;
+  b->dpre = a->activation != MI_ACT_NONE;
+  b->dout = Padded{b->dpre || a->N % 8 != 0 || !at16(a->dout), up8(a->N), 0, 0};
+  if (b->dout.on) {
+    b->dout.at = b->bytes;
+    b->dout.bytes = (size_t)M * b->dout.ld * 2;
+    b->bytes += up256(b->dout.bytes);
+  }
+  if (a->drhs) b->lhs = padded(a->lhs, M, a->K, &b->bytes);
+  if (a->dlhs) {
+    b->rhs = padded(a->rhs, bt ? a->N : a->K, bt ? a->K : a->N, &b->bytes);
+    // dlhs[M,K] = dpre[M,N] . rhs^T: rhs[K,N] is K-contiguous for it, rhs[N,K] is not.
+    const int prc = plan(placed(a->dout, ws, b->dout), b->dout.ld, placed(a->rhs, ws, b->rhs), b->rhs.ld,
+                         bt ? a->N : a->K, a->M, a->K, b->dout.ld, !bt, nullptr, &b->dlhs);
+    if (prc != MI_OK) return prc;
+    b->part_at = b->bytes;
+    b->bytes += up256(b->dlhs.ws_bytes);
+  }
+  if (a->drhs) {
+    b->drhs_padded = a->K % 8 != 0 || a->N % 8 != 0 || !at16(a->drhs);
+    if (b->drhs_padded) {
+      b->drhs_at = b->bytes;
+      b->bytes += up256((size_t)b->kp * up8(a->N) * 2);
+    }
+  }
+  return MI_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int mi_epilogue_num_configs(void) {
+  int n = 0;
+  (void)table(false, &n);
+  return n;
+}
+
+int mi_epilogue_config(int idx, mi_tile_cfg* cfg) {
+  int n = 0;
+  const EpiEntry* t = table(false, &n);
+  if (!cfg) return fail(MI_E_ARGS, "null config");
+  if (idx < 0 || idx >= n) return fail(MI_E_ARGS, "config index %d out of range for the epilogue product", idx);
+  *cfg = t[idx].cfg;
+  return MI_OK;
+}
+
+int mi_epilogue_default_config(int M, int N, int K, int rhs_transposed, mi_tile_cfg* cfg) {
+  if (!cfg) return fail(MI_E_ARGS, "null config");
+  const int rc = check_sizes(M, N, K, MI_ACT_NONE);
+  if (rc != MI_OK) return rc;
+  *cfg = pick(M, N, up8(K), rhs_transposed != 0);
+  return MI_OK;
+}
+
+int mi_matmul_epilogue_workspace(const mi_epilogue_args* a, const mi_tile_cfg* cfg, unsigned long long* bytes) {
+  if (!a || !bytes) return fail(MI_E_ARGS, "null arguments");
+  Fwd f;
+  const int rc = fwd_plan(a, cfg, nullptr, &f);
+  *bytes = rc == MI_OK ? f.bytes : 0;
+  return rc;
+}
+
+int mi_matmul_epilogue_bf16(const mi_epilogue_args* a, const mi_tile_cfg* cfg, void* workspace,
+                            unsigned long long workspace_bytes, void* stream) {
+  if (!a) return fail(MI_E_ARGS, "null arguments");
+  Fwd f;
+  int rc = fwd_plan(a, cfg, (char*)workspace, &f);
+  if (rc != MI_OK) return rc;
+  const int M = a->M, N = a->N, K = a->K;
+  if (M == 0 || N == 0) return MI_OK;
+  if (!a->out || (K > 0 && (!a->lhs || !a->rhs))) return fail(MI_E_ARGS, "null pointer");
+  if (f.bytes && (!workspace || workspace_bytes < f.bytes || !at16(workspace)))
+    return fail(MI_E_ARGS, "the call needs %zu bytes of workspace, 16-byte aligned", f.bytes);
+  if ((uintptr_t)a->lhs % 2 || (uintptr_t)a->rhs % 2 || (uintptr_t)a->out % 2 || (uintptr_t)a->residual % 2 ||
+      (uintptr_t)a->pre % 2 || (uintptr_t)a->bias % (a->bias_f32 ? 4 : 2))
+    return fail(MI_E_ALIGN, "a pointer is not aligned to its elements");
+  const size_t ob = (size_t)M * N * 2;
+  const Range in[] = {{a->lhs, (size_t)M * K * 2}, {a->rhs, (size_t)K * N * 2}, {a->bias, (size_t)N * (a->bias_f32 ? 4 : 2)},
+                      {a->residual, ob}};
+  const Range outs[] = {{a->out, ob}, {a->pre, ob}, {workspace, f.bytes}};
+  if ((rc = check_overlap(outs, in)) != MI_OK) return rc;
+  const hipStream_t s = (hipStream_t)stream;
+  EpiOut o = {};
+  o.bias = a->bias;
+  o.residual = (const uint16_t*)a->residual;
+  o.pre = (uint16_t*)a->pre;
+  o.out = (uint16_t*)a->out;
+  o.M = M;
+  o.N = N;
+  o.act = a->activation;
+  o.bias_f32 = a->bias_f32 != 0;
+  o.vec = N % 8 == 0 && at16(a->bias) && at16(a->residual) && at16(a->pre) && at16(a->out);
+  if (K == 0) {
+    epi_sum_kernel<<<dim3(blocks_for((long long)M * (up8(N) / 8))), dim3(256), 0, s>>>(nullptr, 0, up8(N), o);
+    return launched("epilogue of an empty product");
+  }
+  char* ws = (char*)workspace;
+  const bool bt = a->rhs_transposed != 0;
+  if ((rc = pad(a->lhs, ws, f.lhs, M, K, s)) != MI_OK) return rc;
+  if ((rc = pad(a->rhs, ws, f.rhs, bt ? N : K, bt ? K : N, s)) != MI_OK) return rc;
+  return run(f.mm, o, (float*)(ws + f.part_at), s);
+}
+
+int mi_matmul_epilogue_backward_workspace(const mi_epilogue_grad_args* a, unsigned long long* bytes) {
+  if (!a || !bytes) return fail(MI_E_ARGS, "null arguments");
+  Bwd b;
+  const int rc = bwd_plan(a, nullptr, &b);
+  *bytes = rc == MI_OK ? b.bytes : 0;
+  return rc;
+}
+
+int mi_matmul_epilogue_backward_bf16(const mi_epilogue_grad_args* a, void* workspace,
+                                     unsigned long long workspace_bytes, void* stream) {
+  if (!a) return fail(MI_E_ARGS, "null arguments");
+  Bwd b;
+  int rc = bwd_plan(a, (char*)workspace, &b);
+  if (rc != MI_OK) return rc;
+  const int M = a->M, N = a->N, K = a->K;
+  const bool bt = a->rhs_transposed != 0, act = a->activation != MI_ACT_NONE;
+  const bool any = M > 0 && N > 0;
+  if (any && (!a->dout || (act && !a->pre) || (K > 0 && ((a->dlhs && !a->rhs) || (a->drhs && !a->lhs)))))
+    return fail(MI_E_ARGS, "null pointer");
+  if (b.bytes && (!workspace || workspace_bytes < b.bytes || !at16(workspace)))
+    return fail(MI_E_ARGS, "the call needs %zu bytes of workspace, 16-byte aligned", b.bytes);
+  if ((uintptr_t)a->dout % 2 || (uintptr_t)a->lhs % 2 || (uintptr_t)a->rhs % 2 || (uintptr_t)a->pre % 2 ||
+      (uintptr_t)a->dlhs % 2 || (uintptr_t)a->drhs % 2 || (uintptr_t)a->dbias % (a->bias_f32 ? 4 : 2))
+    return fail(MI_E_ALIGN, "a pointer is not aligned to its elements");
+  const size_t mn = (size_t)M * N * 2, mk = (size_t)M * K * 2, kn = (size_t)K * N * 2;
+  const Range in[] = {{a->dout, mn}, {a->pre, mn}, {a->lhs, mk}, {a->rhs, kn}};
+  const Range outs[] = {{a->dlhs, mk}, {a->drhs, kn}, {a->dbias, (size_t)N * (a->bias_f32 ? 4 : 2)}, {workspace, b.bytes}};
+  if ((rc = check_overlap(outs, in)) != MI_OK) return rc;
+  const hipStream_t s = (hipStream_t)stream;
+  char* ws = (char*)workspace;
+  // Gradients of an empty product or of no rows are zeros; so is dlhs where
+  // rhs has no columns.
+  const auto zeros = [&](void* p, size_t n) {
+    if (!p || n == 0) return (int)MI_OK;
+    mi::fill_zero_kernel<<<dim3(blocks_for((long long)n)), dim3(256), 0, s>>>((uint16_t*)p, n);
+    return launched("zero gradient");
+  };
+  if (!any) {
+    if ((rc = zeros(a->dlhs, (size_t)M * K)) != MI_OK || (rc = zeros(a->drhs, (size_t)K * N)) != MI_OK) return rc;
+    return zeros(a->dbias, (size_t)N * (a->bias_f32 ? 2 : 1));
+  }
+  const uint16_t* dout = (const uint16_t*)a->dout;
+  const uint16_t* dpre = placed(a->dout, ws, b.dout);
+  const int np = up8(N);
+  if (a->dbias || b.dpre) {
+    ActGrad g = {dout, act ? (const uint16_t*)a->pre : nullptr, b.dpre ? (uint16_t*)dpre : nullptr,
+                 a->dbias ? (float*)(ws + b.bias_at) : nullptr, M, N, np, a->activation,
+                 N % 8 == 0 && at16(a->dout) && at16(a->pre)};
+    const int xb = (np + 511) / 512, rows4 = (M + 3) / 4;
+    int chunks = a->dbias ? b.chunks : 4096 / xb;
+    chunks = chunks < 1 ? 1 : chunks > rows4 ? rows4 : chunks;
+    act_grad_kernel<<<dim3((unsigned)xb, (unsigned)chunks), dim3(256), 0, s>>>(g);
+    if ((rc = launched("activation gradient")) != MI_OK) return rc;
+    if (a->dbias) {
+      const mi::ColumnSum c = {g.part, {a->dbias, nullptr}, chunks, N};
+      const dim3 grid((unsigned)((N + 63) / 64), 1);
+      if (a->bias_f32) mi::column_sum_kernel<float><<<grid, dim3(1024), 0, s>>>(c);
+      else mi::column_sum_kernel<mi::Bf16><<<grid, dim3(1024), 0, s>>>(c);
+      if ((rc = launched("bias gradient")) != MI_OK) return rc;
+    }
+  }
+  if (K == 0) return MI_OK;
+  if (!b.dpre && (a->dlhs || a->drhs) && (rc = pad(a->dout, ws, b.dout, M, N, s)) != MI_OK) return rc;
+  if (a->dlhs) {
+    if ((rc = pad(a->rhs, ws, b.rhs, bt ? N : K, bt ? K : N, s)) != MI_OK) return rc;
+    EpiOut o = {};
+    o.out = (uint16_t*)a->dlhs;
+    o.M = M;
+    o.N = K;
+    o.vec = K % 8 == 0 && at16(a->dlhs);
+    if ((rc = run(b.dlhs, o, (float*)(ws + b.part_at), s)) != MI_OK) return rc;
+  }
+  if (a->drhs) {
+    if ((rc = pad(a->lhs, ws, b.lhs, M, K, s)) != MI_OK) return rc;
+    const uint16_t* lhs = placed(a->lhs, ws, b.lhs);
+    uint16_t* out = (uint16_t*)(b.drhs_padded ? (void*)(ws + b.drhs_at) : a->drhs);
+    // drhs[K,N] = lhs^T . dpre, or drhs[N,K] = dpre^T . lhs: rows M contracted.
+    rc = bt ? mi::capi::matmul_lhsT_rhs_bf16(dpre, lhs, out, np, b.kp, M, nullptr, stream, nullptr, 0)
+            : mi::capi::matmul_lhsT_rhs_bf16(lhs, dpre, out, b.kp, np, M, nullptr, stream, nullptr, 0);
+    if (rc != MI_OK) return rc;
+    if (b.drhs_padded) {
+      const long long rows = bt ? N : K;
+      const int c = bt ? K : N;
+      unpad_rows_kernel<<<dim3(blocks_for(rows * c)), dim3(256), 0, s>>>(out, (uint16_t*)a->drhs, rows, c, up8(c));
+      return launched("gradient's copy");
+    }
+  }
+  return MI_OK;
+}
+
+}  // extern "C"

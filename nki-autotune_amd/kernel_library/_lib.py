@@ -34,6 +34,16 @@ MI_E_KERNEL = 7
 MI_E_SPLIT = 8
 MI_E_TILE = 9
 
+# Element types and activations of the operators with argument structures.
+MI_DTYPE_BF16 = 0
+MI_DTYPE_F16 = 1
+MI_DTYPE_F32 = 2
+MI_ACT_NONE = 0
+MI_ACT_RELU = 1
+MI_ACT_GELU = 2
+MI_ACT_GELU_TANH = 3
+MI_ACT_SILU = 4
+
 CODE_NAMES = {
     MI_E_NO_INSTANCE: "no compiled instance",
     MI_E_LDS: "LDS over budget",
@@ -58,6 +68,16 @@ EXPORTED_SYMBOLS = (
     "mi_matmul_lhs_rhs_bf16",
     "mi_matmul_lhsT_rhs_f32",
     "mi_rmsnorm_matmul_bf16",
+    "mi_layer_norm",
+    "mi_layer_norm_backward",
+    "mi_layer_norm_backward_workspace",
+    "mi_epilogue_num_configs",
+    "mi_epilogue_config",
+    "mi_epilogue_default_config",
+    "mi_matmul_epilogue_bf16",
+    "mi_matmul_epilogue_workspace",
+    "mi_matmul_epilogue_backward_bf16",
+    "mi_matmul_epilogue_backward_workspace",
     "mi_device_info",
     "mi_release_workspace",
     "mi_last_error",
@@ -67,7 +87,19 @@ EXPORTED_SYMBOLS = (
 
 # Exported by libmi_kernels.so only (not by the single-config libraries the
 # autotuner builds just in time).
-PREBUILT_ONLY_SYMBOLS = frozenset({"mi_matmul_lhsT_rhs_bf16_noalloc"})
+PREBUILT_ONLY_SYMBOLS = frozenset({
+    "mi_matmul_lhsT_rhs_bf16_noalloc",
+    "mi_layer_norm",
+    "mi_layer_norm_backward",
+    "mi_layer_norm_backward_workspace",
+    "mi_epilogue_num_configs",
+    "mi_epilogue_config",
+    "mi_epilogue_default_config",
+    "mi_matmul_epilogue_bf16",
+    "mi_matmul_epilogue_workspace",
+    "mi_matmul_epilogue_backward_bf16",
+    "mi_matmul_epilogue_backward_workspace",
+})
 # Bytes of the static device scratch of mi_matmul_lhsT_rhs_bf16_noalloc
 # (MI_NOALLOC_SCRATCH_BYTES).
 NOALLOC_SCRATCH_BYTES = 64 << 20
@@ -88,6 +120,35 @@ class MiTileCfg(ctypes.Structure):
     ]
 
 
+def _fields(ptrs: str, longs: str = "", ints: str = "", floats: str = "") -> list:
+    return [(n, t) for names, t in ((ptrs, ctypes.c_void_p), (longs, ctypes.c_longlong), (ints, ctypes.c_int),
+                                    (floats, ctypes.c_float)) for n in names.split()]
+
+
+class LayerNormArgs(ctypes.Structure):
+    """``mi_layer_norm_args`` of include/mi_kernels.h."""
+
+    _fields_ = _fields("x weight bias y mean rstd", "rows ldx", "D dtype params_f32", "eps")
+
+
+class LayerNormGradArgs(ctypes.Structure):
+    """``mi_layer_norm_grad_args`` of include/mi_kernels.h."""
+
+    _fields_ = _fields("dout x weight mean rstd dx dweight dbias", "rows lddout ldx", "D dtype params_f32")
+
+
+class EpilogueArgs(ctypes.Structure):
+    """``mi_epilogue_args`` of include/mi_kernels.h."""
+
+    _fields_ = _fields("lhs rhs bias residual out pre", ints="M N K rhs_transposed activation bias_f32")
+
+
+class EpilogueGradArgs(ctypes.Structure):
+    """``mi_epilogue_grad_args`` of include/mi_kernels.h."""
+
+    _fields_ = _fields("dout lhs rhs pre dlhs drhs dbias", ints="M N K rhs_transposed activation bias_f32")
+
+
 class KernelLibraryError(RuntimeError):
     """A launch or legality failure reported by libmi_kernels.so."""
 
@@ -103,6 +164,9 @@ _LIBS: dict[str, ctypes.CDLL] = {}
 def _declare(lib: ctypes.CDLL) -> None:
     c_int, c_void_p, c_float, c_char_p = ctypes.c_int, ctypes.c_void_p, ctypes.c_float, ctypes.c_char_p
     cfgp = ctypes.POINTER(MiTileCfg)
+    c_u64, u64p = ctypes.c_ulonglong, ctypes.POINTER(ctypes.c_ulonglong)
+    lnp, lngp = ctypes.POINTER(LayerNormArgs), ctypes.POINTER(LayerNormGradArgs)
+    epp, epgp = ctypes.POINTER(EpilogueArgs), ctypes.POINTER(EpilogueGradArgs)
     sigs = {
         "mi_cfg_check": (c_int, [c_int, cfgp, c_int, c_int, c_int]),
         "mi_num_configs": (c_int, [c_int]),
@@ -120,6 +184,16 @@ def _declare(lib: ctypes.CDLL) -> None:
             c_int,
             [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_float, cfgp, c_void_p],
         ),
+        "mi_layer_norm": (c_int, [lnp, c_void_p]),
+        "mi_layer_norm_backward": (c_int, [lngp, c_void_p, c_u64, c_void_p]),
+        "mi_layer_norm_backward_workspace": (c_int, [lngp, u64p]),
+        "mi_epilogue_num_configs": (c_int, []),
+        "mi_epilogue_config": (c_int, [c_int, cfgp]),
+        "mi_epilogue_default_config": (c_int, [c_int, c_int, c_int, c_int, cfgp]),
+        "mi_matmul_epilogue_bf16": (c_int, [epp, cfgp, c_void_p, c_u64, c_void_p]),
+        "mi_matmul_epilogue_workspace": (c_int, [epp, cfgp, u64p]),
+        "mi_matmul_epilogue_backward_bf16": (c_int, [epgp, c_void_p, c_u64, c_void_p]),
+        "mi_matmul_epilogue_backward_workspace": (c_int, [epgp, u64p]),
         "mi_device_info": (c_int, [ctypes.POINTER(c_int), c_char_p, c_int, ctypes.POINTER(c_int)]),
         "mi_release_workspace": (c_int, []),
         "mi_last_error": (c_char_p, []),

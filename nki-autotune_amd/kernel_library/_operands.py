@@ -1,0 +1,63 @@
+"""Argument checks, workspaces and launches shared by the operators that take argument structures."""
+
+from __future__ import annotations
+
+import ctypes
+from collections.abc import Callable, Container
+
+import torch
+
+from kernel_library import _lib
+
+
+def tensor(name: str, t: object, dtypes: Container[torch.dtype], ref: torch.Tensor | None = None,
+           ref_name: str = "") -> None:
+    """``t`` is a tensor of one of ``dtypes`` on a HIP device (``ref``'s, where given)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor on a HIP device, got {type(t).__name__}")
+    if t.device.type != "cuda":
+        raise ValueError(f"{name} must live on a HIP device (got {t.device})")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name} dtype {t.dtype} not in {tuple(dtypes)}")
+    if ref is not None and t.device != ref.device:
+        raise ValueError(f"{name} is on {t.device}, {ref_name} on {ref.device}: all operands must share a device")
+
+
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """The first byte of ``t`` and the one past its last."""
+    if t.numel() == 0:
+        return 0, 0
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def no_overlap(name: str, out: torch.Tensor, **others: torch.Tensor | None) -> None:
+    """``out`` shares no bytes with another operand: the kernels read those while they write ``out``."""
+    o0, o1 = _span(out)
+    for other, t in others.items():
+        if t is None:
+            continue
+        t0, t1 = _span(t)
+        if t0 < o1 and o0 < t1:
+            raise ValueError(f"{name} overlaps {other}: an output must not alias another operand")
+
+
+def workspace(device: torch.device, what: str, query: Callable, *args) -> tuple[torch.Tensor | None, int]:
+    """The workspace that a call needs, and its bytes: from torch's allocator on the current stream, so that calls on
+    several streams, and graphs, have one each."""
+    need = ctypes.c_ulonglong()
+    _lib.check_rc(query(*args, ctypes.byref(need)), what)
+    if not need.value:
+        return None, 0
+    return torch.empty(need.value, dtype=torch.uint8, device=device), need.value
+
+
+def launch(device: torch.device, what: str, fn: Callable, *args) -> None:
+    """``fn(*args, stream)`` on the current stream of ``device``."""
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, stream)
+    _lib.check_rc(rc, what)
