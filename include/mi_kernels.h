@@ -320,6 +320,22 @@ int mi_matmul_epilogue_backward_workspace(const mi_epilogue_grad_args* args, uns
 int mi_matmul_epilogue_backward_bf16(const mi_epilogue_grad_args* args, void* workspace,
                                      unsigned long long workspace_bytes, void* stream);
 
+/* out = the Newton-Schulz iterate of each of `batch` matrices grad [m,n]
+ * (bf16 or fp32, contiguous) after `steps` steps, bf16: X = grad /
+ * (||grad||_F + eps), turned where m > n; then steps times A = X X^T, X =
+ * a X + (b A + c A A) X.  The iterates are held in 16 bits of mantissa (two
+ * bf16) and the products accumulate in fp32.  Any sizes; a matrix's planes
+ * (4 bytes an element, the longer side rounded up to 64) under 4 GiB,
+ * at most 65535 matrices (MI_E_RANGE). */
+typedef struct {
+  const void* grad;
+  void* out;
+  int batch, m, n, steps, dtype;
+  float a, b, c, eps;
+} mi_newton_schulz_args;
+int mi_newton_schulz_workspace(const mi_newton_schulz_args* args, unsigned long long* bytes);
+int mi_newton_schulz(const mi_newton_schulz_args* args, void* workspace, unsigned long long workspace_bytes, void* stream);
+
 /* Device discovery: number of visible HIP devices and the gfx arch name of
  * device 0 (written to arch, at most arch_len bytes).  Returns 0 or -error.
  * Replaces detect_neuron_cores()

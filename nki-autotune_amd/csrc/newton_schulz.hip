@@ -1,0 +1,241 @@
+// newton_schulz.hip -- mi_newton_schulz: argument checks, workspace, and the
+// launches of its products (mi_ns.hpp).
+#include "mi_capi_internal.hpp"
+#include "mi_norm.hpp"
+#include "mi_ns.hpp"
+
+namespace {
+
+using mi::Bf16;
+using mi::EpiMM;
+using mi::NsOut;
+using mi::capi::fail;
+
+constexpr int kNormBlocks = 256;  // blocks of one matrix's sum of squares
+
+// part[z][block] = the sum of squares of a share of G_z, in 64 bits (the
+// squares of small gradients leave fp32's range).
+template <class T>
+__global__ __launch_bounds__(256) void ns_square_kernel(const T* __restrict__ g, double* __restrict__ part, long long n) {
+  __shared__ double xs[4];
+  const T* p = g + (size_t)blockIdx.y * (size_t)n;
+  double s = 0.0;
+  constexpr int U = 8;
+  const long long step = (long long)gridDim.x * 256;
+  for (long long i0 = (long long)blockIdx.x * 256 + threadIdx.x; i0 < n; i0 += U * step) {
+    float v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = i0 + u * step < n ? mi::to_f32(p[i0 + u * step]) : 0.0f;
+#pragma unroll
+    for (int u = 0; u < U; ++u) s += (double)v[u] * (double)v[u];
+  }
+#pragma unroll
+  for (int k = 32; k > 0; k >>= 1) s += __shfl_xor(s, k);
+  if ((threadIdx.x & 63) == 0) xs[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) part[(size_t)blockIdx.y * gridDim.x + blockIdx.x] = ((xs[0] + xs[1]) + xs[2]) + xs[3];
+}
+
+// The planes of X_0 = G / (||G|| + eps), or of G^T: 64 x 64 pieces, turned in
+// LDS.  G [m][n]; X [s][2 * lp], s x l of it G's or G^T's, the rest zeros.
+struct NsInit {
+  const void* g;
+  uint16_t* x;
+  const double* part;
+  int parts, m, n, s, l, lp;
+  float eps;
+  bool turn;
+};
+template <class T>
+__global__ __launch_bounds__(256) void ns_init_kernel(const NsInit p) {
+  __shared__ float tile[64][65];
+  __shared__ double sums[kNormBlocks];
+  __shared__ float scale_lds;
+  const int tid = (int)threadIdx.x, z = (int)blockIdx.z;
+  if (tid < p.parts) sums[tid] = p.part[(size_t)z * p.parts + tid];
+  const T* g = (const T*)p.g + (size_t)z * (size_t)p.m * (size_t)p.n;
+  const int r0 = (int)blockIdx.y * 64, c0 = (int)blockIdx.x * 64;  // of X
+  for (int i = tid; i < 64 * 64; i += 256) {
+    const int a = i / 64, b = i % 64;
+    const int row = (p.turn ? c0 : r0) + a, col = (p.turn ? r0 : c0) + b;  // of G
+    const float v = row < p.m && col < p.n ? mi::to_f32(g[(size_t)row * (size_t)p.n + col]) : 0.0f;
+    if (p.turn) tile[b][a] = v;
+    else tile[a][b] = v;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    double t = 0.0;
+    for (int i = 0; i < p.parts; ++i) t += sums[i];
+    scale_lds = (float)(1.0 / (__builtin_sqrt(t) + (double)p.eps));
+  }
+  __syncthreads();
+  const float scale = scale_lds;
+  uint16_t* x = p.x + (size_t)z * (size_t)p.s * (size_t)(2 * p.lp);
+  for (int i = tid; i < 64 * 8; i += 256) {
+    const int r = i / 8, c = (i % 8) * 8;
+    if (r0 + r >= p.s) continue;
+    float v[8], t[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = tile[r][c + k] * scale;
+    const mi::u32x4_t hi = mi::pack8(v);
+    mi::unpack8(hi, t);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] -= t[k];
+    uint16_t* at = x + (size_t)(r0 + r) * (size_t)(2 * p.lp) + c0 + c;
+    *(mi::u32x4_t*)at = hi;
+    *(mi::u32x4_t*)(at + p.lp) = mi::pack8(v);
+  }
+}
+
+// out [m][n] from the hi plane of X [s][2 * lp], turned back where G was.
+// hi is the value rounded to bf16.
+__global__ __launch_bounds__(256) void ns_last_kernel(const uint16_t* __restrict__ x, uint16_t* __restrict__ out, int m,
+                                                      int n, int s, int lp, bool turn) {
+  __shared__ uint16_t tile[64][66];
+  const int tid = (int)threadIdx.x, z = (int)blockIdx.z;
+  const int r0 = (int)blockIdx.y * 64, c0 = (int)blockIdx.x * 64;  // of out
+  const uint16_t* src = x + (size_t)z * (size_t)s * (size_t)(2 * lp);
+  for (int i = tid; i < 64 * 64; i += 256) {
+    const int a = i / 64, b = i % 64;
+    const int row = (turn ? c0 : r0) + a, col = (turn ? r0 : c0) + b;  // of X
+    const bool in = row < s && col < lp;
+    const uint16_t v = in ? src[(size_t)row * (size_t)(2 * lp) + col] : (uint16_t)0;
+    if (turn) tile[b][a] = v;
+    else tile[a][b] = v;
+  }
+  __syncthreads();
+  uint16_t* dst = out + (size_t)z * (size_t)m * (size_t)n;
+  for (int i = tid; i < 64 * 64; i += 256) {
+    const int r = r0 + i / 64, c = c0 + i % 64;
+    if (r < m && c < n) dst[(size_t)r * (size_t)n + c] = tile[i / 64][i % 64];
+  }
+}
+
+int launched(const char* what) {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? MI_OK : fail(-(int)e, "%s: %s", what, hipGetErrorString(e));
+}
+
+size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+
+struct Plan {
+  int s, l, sp, lp, parts;
+  bool turn;
+  size_t x0, x1, a, b, part, bytes;
+};
+int ns_plan(const mi_newton_schulz_args* p, Plan* q) {
+  if (p->batch < 0 || p->m < 0 || p->n < 0) return fail(MI_E_ARGS, "negative size batch=%d m=%d n=%d", p->batch, p->m, p->n);
+  if (p->steps < 0) return fail(MI_E_ARGS, "steps=%d negative", p->steps);
+  if (p->dtype != MI_DTYPE_BF16 && p->dtype != MI_DTYPE_F32) return fail(MI_E_ARGS, "grad must be bf16 or fp32");
+  if (!(p->eps >= 0.0f) || p->eps > 3.0e38f) return fail(MI_E_ARGS, "eps must be finite and >= 0");
+  if (p->batch > 65535) return fail(MI_E_RANGE, "batch=%d over 65535", p->batch);
+  *q = Plan{};
+  if (p->batch == 0 || p->m == 0 || p->n == 0) return MI_OK;
+  q->turn = p->m > p->n;
+  q->s = q->turn ? p->n : p->m;
+  q->l = q->turn ? p->m : p->n;
+  // A matrix's planes, and a block of rows past them, within 32-bit offsets.
+  const unsigned long long lp = ((unsigned long long)q->l + 63) / 64 * 64;
+  if (((unsigned long long)q->s + 512) * lp * 4 > mi::capi::kMaxOffset)
+    return fail(MI_E_RANGE, "the planes of a %d x %d matrix exceed 32-bit buffer offsets", p->m, p->n);
+  if (lp / 64 > 65535) return fail(MI_E_RANGE, "a side of %d exceeds 64 * 65535", q->l);
+  q->lp = (int)lp;
+  q->sp = (q->s + 63) / 64 * 64;
+  const long long n = (long long)p->m * p->n;
+  q->parts = (int)(n / 2048 < 1 ? 1 : n / 2048 > kNormBlocks ? kNormBlocks : n / 2048);
+  const size_t x = up256((size_t)p->batch * q->s * q->lp * 4), a = up256((size_t)p->batch * q->s * q->sp * 4);
+  q->x1 = x;
+  q->a = 2 * x;
+  q->b = q->a + a;
+  q->part = q->b + a;
+  q->bytes = q->part + up256((size_t)p->batch * q->parts * 8);
+  return MI_OK;
+}
+
+template <int BM, int BN, int BK, int W, int S, bool BT>
+int product(const EpiMM& p, const NsOut& o, int batch, hipStream_t s) {
+  const unsigned tiles = (unsigned)((p.M + BM - 1) / BM) * (unsigned)((p.N + BN - 1) / BN);
+  mi::ns_product_kernel<BM, BN, BK, W, S, BT><<<dim3(tiles, (unsigned)batch), dim3(W * 64), 0, s>>>(p, o);
+  return launched("Newton-Schulz product");
+}
+template <bool BT>
+int product(const EpiMM& p, const NsOut& o, int batch, hipStream_t s) {
+  const auto tiles = [&](int b) { return (long long)batch * ((p.M + b - 1) / b) * ((p.N + b - 1) / b); };
+  if (tiles(256) >= 200) return product<256, 256, 64, 8, 2, BT>(p, o, batch, s);
+  if (tiles(128) >= 200) return product<128, 128, 64, 4, 4, BT>(p, o, batch, s);
+  return product<64, 64, 64, 4, 4, BT>(p, o, batch, s);
+}
+
+}  // namespace
+
+extern "C" {
+
+int mi_newton_schulz_workspace(const mi_newton_schulz_args* args, unsigned long long* bytes) {
+  if (!args || !bytes) return fail(MI_E_ARGS, "null arguments");
+  Plan q;
+  const int rc = ns_plan(args, &q);
+  *bytes = rc == MI_OK ? q.bytes : 0;
+  return rc;
+}
+
+int mi_newton_schulz(const mi_newton_schulz_args* args, void* workspace, unsigned long long workspace_bytes, void* stream) {
+  if (!args) return fail(MI_E_ARGS, "null arguments");
+  Plan q;
+  int rc = ns_plan(args, &q);
+  if (rc != MI_OK || q.bytes == 0) return rc;
+  const int m = args->m, n = args->n, batch = args->batch;
+  const size_t es = args->dtype == MI_DTYPE_F32 ? 4 : 2, total = (size_t)batch * m * n;
+  if (!args->grad || !args->out) return fail(MI_E_ARGS, "null pointer");
+  if (!workspace || workspace_bytes < q.bytes || (uintptr_t)workspace % 16)
+    return fail(MI_E_ARGS, "the call needs %zu bytes of workspace, 16-byte aligned", q.bytes);
+  if ((uintptr_t)args->grad % es || (uintptr_t)args->out % 2) return fail(MI_E_ALIGN, "a pointer is not aligned to its elements");
+  const auto overlap = [](const void* a, size_t ab, const void* b, size_t bb) {
+    return (uintptr_t)a < (uintptr_t)b + bb && (uintptr_t)b < (uintptr_t)a + ab;
+  };
+  if (overlap(args->grad, total * es, args->out, total * 2) || overlap(workspace, q.bytes, args->grad, total * es) ||
+      overlap(workspace, q.bytes, args->out, total * 2))
+    return fail(MI_E_ARGS, "out overlaps grad, or the workspace one of them");
+  const hipStream_t st = (hipStream_t)stream;
+  char* ws = (char*)workspace;
+  double* part = (double*)(ws + q.part);
+  uint16_t *x = (uint16_t*)ws, *next = (uint16_t*)(ws + q.x1), *A = (uint16_t*)(ws + q.a), *B = (uint16_t*)(ws + q.b);
+  const long long per = (long long)m * n;
+  const dim3 sq((unsigned)q.parts, (unsigned)batch);
+  const NsInit init = {args->grad, x, part, q.parts, m, n, q.s, q.l, q.lp, args->eps, q.turn};
+  const dim3 ig((unsigned)(q.lp / 64), (unsigned)((q.s + 63) / 64), (unsigned)batch);
+  if (args->dtype == MI_DTYPE_F32) {
+    ns_square_kernel<float><<<sq, dim3(256), 0, st>>>((const float*)args->grad, part, per);
+    if ((rc = launched("sum of squares")) != MI_OK) return rc;
+    ns_init_kernel<float><<<ig, dim3(256), 0, st>>>(init);
+  } else {
+    ns_square_kernel<Bf16><<<sq, dim3(256), 0, st>>>((const Bf16*)args->grad, part, per);
+    if ((rc = launched("sum of squares")) != MI_OK) return rc;
+    ns_init_kernel<Bf16><<<ig, dim3(256), 0, st>>>(init);
+  }
+  if ((rc = launched("first iterate")) != MI_OK) return rc;
+  const int s = q.s, sp = q.sp, lp = q.lp;
+  const uint32_t xb = (uint32_t)((size_t)s * lp * 4), ab = (uint32_t)((size_t)s * sp * 4);
+  const long long xz = (long long)s * lp * 2, az = (long long)s * sp * 2;
+  const bool direct = !q.turn && n == lp && (uintptr_t)args->out % 16 == 0;  // the last product stores out itself
+  for (int k = 0; k < args->steps; ++k) {
+    const EpiMM gram = {x, x, xb, xb, s, sp, lp, 2 * lp, 2 * lp, 8, 1, (uint32_t)lp * 2, (uint32_t)lp * 2, xz, xz};
+    const NsOut to_a = {nullptr, A, nullptr, s, sp, 2 * sp, 1.0f, 0.0f, 0, az};
+    if ((rc = product<true>(gram, to_a, batch, st)) != MI_OK) return rc;
+    const EpiMM square = {A, A, ab, ab, s, sp, sp, 2 * sp, 2 * sp, 8, 1, (uint32_t)sp * 2, (uint32_t)sp * 2, az, az};
+    const NsOut to_b = {A, B, nullptr, s, sp, 2 * sp, args->c, args->b, az, az};
+    if ((rc = product<true>(square, to_b, batch, st)) != MI_OK) return rc;
+    const EpiMM update = {B, x, ab, xb, s, lp, sp, 2 * sp, 2 * lp, 8, 1, (uint32_t)sp * 2, (uint32_t)lp * 2, az, xz};
+    const bool last = direct && k + 1 == args->steps;
+    const NsOut to_x = {x, next, last ? (uint16_t*)args->out : nullptr, s, lp, 2 * lp, 1.0f, args->a, xz, last ? per : xz};
+    if ((rc = product<false>(update, to_x, batch, st)) != MI_OK) return rc;
+    uint16_t* t = x;
+    x = next;
+    next = t;
+    if (last) return MI_OK;
+  }
+  const dim3 lg((unsigned)((n + 63) / 64), (unsigned)((m + 63) / 64), (unsigned)batch);
+  ns_last_kernel<<<lg, dim3(256), 0, st>>>(x, (uint16_t*)args->out, m, n, s, lp, q.turn);
+  return launched("last iterate");
+}
+
+}  // extern "C"

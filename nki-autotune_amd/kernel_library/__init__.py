@@ -6,6 +6,7 @@ Public kernels (torch device tensors in, torch device tensor out):
 * :func:`matmul_lhs_rhs` -- ``lhs[M,K] @ rhs[K,N]``, bf16
 * :func:`rmsnorm_matmul` -- ``rmsnorm(lhs) * gamma @ rhs``, bf16
 * :func:`matmul_epilogue` -- ``act(lhs @ rhs + bias) + residual``, bf16, and :func:`matmul_epilogue_backward`
+* :func:`newton_schulz` -- an update matrix orthogonalised (the Muon optimiser's step), bf16 or fp32
 * :func:`layer_norm` -- bf16, fp16 or fp32, and :func:`layer_norm_backward`
 
 plus the reference names ``matmul_lhsT_rhs_nkigym``, ``matmul_lhs_rhs_nkigym`` and
@@ -23,6 +24,7 @@ from kernel_library.config import (
 )
 from kernel_library.epilogue import epilogue_configs, matmul_epilogue, matmul_epilogue_backward
 from kernel_library.norm import layer_norm, layer_norm_backward
+from kernel_library.orthogonal import newton_schulz
 from kernel_library.ops import (
     EPS,
     matmul_lhs_rhs,
@@ -48,6 +50,7 @@ __all__ = [
     "matmul_epilogue",
     "matmul_epilogue_backward",
     "matmul_lhs_rhs",
+    "newton_schulz",
     "matmul_lhs_rhs_nkigym",
     "matmul_lhsT_rhs",
     "matmul_lhsT_rhs_nkigym",

@@ -78,6 +78,8 @@ EXPORTED_SYMBOLS = (
     "mi_matmul_epilogue_workspace",
     "mi_matmul_epilogue_backward_bf16",
     "mi_matmul_epilogue_backward_workspace",
+    "mi_newton_schulz",
+    "mi_newton_schulz_workspace",
     "mi_device_info",
     "mi_release_workspace",
     "mi_last_error",
@@ -99,6 +101,8 @@ PREBUILT_ONLY_SYMBOLS = frozenset({
     "mi_matmul_epilogue_workspace",
     "mi_matmul_epilogue_backward_bf16",
     "mi_matmul_epilogue_backward_workspace",
+    "mi_newton_schulz",
+    "mi_newton_schulz_workspace",
 })
 # Bytes of the static device scratch of mi_matmul_lhsT_rhs_bf16_noalloc
 # (MI_NOALLOC_SCRATCH_BYTES).
@@ -149,6 +153,12 @@ class EpilogueGradArgs(ctypes.Structure):
     _fields_ = _fields("dout lhs rhs pre dlhs drhs dbias", ints="M N K rhs_transposed activation bias_f32")
 
 
+class NewtonSchulzArgs(ctypes.Structure):
+    """``mi_newton_schulz_args`` of include/mi_kernels.h."""
+
+    _fields_ = _fields("grad out", ints="batch m n steps dtype", floats="a b c eps")
+
+
 class KernelLibraryError(RuntimeError):
     """A launch or legality failure reported by libmi_kernels.so."""
 
@@ -194,6 +204,8 @@ def _declare(lib: ctypes.CDLL) -> None:
         "mi_matmul_epilogue_workspace": (c_int, [epp, cfgp, u64p]),
         "mi_matmul_epilogue_backward_bf16": (c_int, [epgp, c_void_p, c_u64, c_void_p]),
         "mi_matmul_epilogue_backward_workspace": (c_int, [epgp, u64p]),
+        "mi_newton_schulz": (c_int, [ctypes.POINTER(NewtonSchulzArgs), c_void_p, c_u64, c_void_p]),
+        "mi_newton_schulz_workspace": (c_int, [ctypes.POINTER(NewtonSchulzArgs), u64p]),
         "mi_device_info": (c_int, [ctypes.POINTER(c_int), c_char_p, c_int, ctypes.POINTER(c_int)]),
         "mi_release_workspace": (c_int, []),
         "mi_last_error": (c_char_p, []),

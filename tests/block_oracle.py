@@ -115,3 +115,17 @@ def within(actual: torch.Tensor, expected: torch.Tensor, tol) -> None:
         i = tuple(at)
         raise AssertionError(f"{int((~ok).sum())} of {e.numel()} values off; first at {at}: got {float(a[i])!r}, "
                              f"expected {float(e[i])!r} within {float(tol[i])!r}")
+
+
+def newton_schulz(grad, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
+    """The iterate after ``steps`` steps in float64, of each matrix of a batch."""
+    if grad.dim() == 3:
+        return torch.stack([newton_schulz(g, steps, coefficients, eps) for g in grad])
+    a, b, c = coefficients
+    turn = grad.shape[0] > grad.shape[1]
+    x = grad.double().t().contiguous() if turn else grad.double()
+    x = x / (torch.linalg.norm(x) + eps)
+    for _ in range(steps):
+        A = x @ x.t().contiguous()
+        x = a * x + (b * A + c * (A @ A)) @ x
+    return x.t().contiguous() if turn else x
