@@ -49,10 +49,10 @@ __global__ __launch_bounds__(256) void epi_sum_kernel(const float* __restrict__ 
   const int groups = ldw / 8;
   const long long n = (long long)e.M * groups;
   const size_t stride = (size_t)e.M * (size_t)ldw;
+  e.m0 = 0;
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
     const int m = (int)(i / groups), c = (int)(i - (long long)m * groups) * 8;
     e.columns(c);
-    e.fetch(0, m, c);
     float v[8] = {};
     if (parts > 0) {
       const float* at = ws + (size_t)m * (size_t)ldw + c;
@@ -415,7 +415,8 @@ int mi_matmul_epilogue_bf16(const mi_epilogue_args* a, const mi_tile_cfg* cfg, v
   o.N = N;
   o.act = a->activation;
   o.bias_f32 = a->bias_f32 != 0;
-  o.vec = N % 8 == 0 && at16(a->bias) && at16(a->residual) && at16(a->pre) && at16(a->out);
+  // (A block's rows of the outputs are within 32-bit offsets up to a million columns.)
+  o.vec = N % 8 == 0 && N <= 1 << 20 && at16(a->bias) && at16(a->residual) && at16(a->pre) && at16(a->out);
   if (K == 0) {
     epi_sum_kernel<<<dim3(blocks_for((long long)M * (up8(N) / 8))), dim3(256), 0, s>>>(nullptr, 0, up8(N), o);
     return launched("epilogue of an empty product");
@@ -496,7 +497,7 @@ int mi_matmul_epilogue_backward_bf16(const mi_epilogue_grad_args* a, void* works
     o.out = (uint16_t*)a->dlhs;
     o.M = M;
     o.N = K;
-    o.vec = K % 8 == 0 && at16(a->dlhs);
+    o.vec = K % 8 == 0 && K <= 1 << 20 && at16(a->dlhs);
     if ((rc = run(b.dlhs, o, (float*)(ws + b.part_at), s)) != MI_OK) return rc;
   }
   if (a->drhs) {

@@ -6,18 +6,23 @@
 // block_m, block_n, block_k, waves, lds_stages, rhs read non-temporally
 #define MI_EPI_CONFIGS(X)   \
   X(256, 256, 64, 8, 2, 0)  \
-  X(256, 256, 64, 4, 2, 0)  \
   X(256, 128, 64, 8, 3, 0)  \
+  X(256, 128, 64, 4, 2, 0)  \
+  X(256, 128, 64, 8, 2, 0)  \
   X(128, 256, 64, 8, 3, 0)  \
-  X(128, 256, 64, 4, 3, 0)  \
+  X(128, 256, 64, 4, 2, 0)  \
   X(128, 128, 64, 4, 2, 0)  \
   X(128, 128, 64, 4, 4, 0)  \
+  X(64, 128, 64, 4, 2, 0)   \
   X(64, 128, 64, 4, 3, 0)   \
+  X(128, 64, 64, 4, 2, 0)   \
   X(128, 64, 64, 4, 3, 0)   \
+  X(64, 64, 64, 4, 2, 0)    \
   X(64, 64, 64, 4, 4, 0)    \
   X(32, 64, 64, 2, 4, 0)    \
   X(32, 128, 64, 4, 4, 1)   \
   X(64, 128, 64, 4, 4, 1)   \
+  X(128, 128, 64, 4, 2, 1)  \
   X(128, 128, 64, 4, 3, 1)
 
 namespace mi {

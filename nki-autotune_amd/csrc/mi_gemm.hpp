@@ -323,14 +323,13 @@ struct KPanelLoader {
       lds_off[j] = c * 1024;
     }
   }
-  template <bool NT = false>
   __device__ __forceinline__ void issue_at(int j, __amdgpu_buffer_rsrc_t rs_kt, char* smem, int base,
                                            bool tail) const {
     // One load either way, its offset selected without a branch: a branch
     // per load splits the main loop into blocks, and code the compiler
     // moves between blocks (sinking a chain of VALU work into the last
     // block of the loop body) escapes the scheduling hints of its sub-step.
-    if (EVEN || active[j]) lds_dma16<NT>(rs_kt, smem + base + lds_off[j], tail ? voff_tail[j] : voff[j]);
+    if (EVEN || active[j]) lds_dma16(rs_kt, smem + base + lds_off[j], tail ? voff_tail[j] : voff[j]);
   }
   static constexpr int LOADS_PER_TILE = PER_WAVE;
 };

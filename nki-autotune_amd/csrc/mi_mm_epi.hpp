@@ -41,33 +41,101 @@ struct EpiMM {
   long long batch_a, batch_b;         // elements from one product's operand to the next's (blockIdx.y)
 };
 
+// TM x TN fragments of 16 rows and 16 columns a wave.
 template <int BM, int BN, int BK, int WAVES, int STAGES>
 struct EpiCfg {
   using G = WaveGrid<BM, BN, WAVES>;
+  static constexpr int TM = G::WTM / 16, TN = G::WTN / 16;
   static constexpr int A_BYTES = BK * BM * 2;
   static constexpr int B_BYTES = BK * BN * 2;
-  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int TURN_COLS = G::TN >= 2 ? 64 : 32;
+  // The stages of A, then those of B: an LDS read's offset from a lane's
+  // address then fits its 16 bits (with A and B of a stage together, the
+  // second stage of a 256x256 block took a register per read).
+  static constexpr int B_OFF = STAGES * A_BYTES;
+  static constexpr int TURN_COLS = TN >= 4 ? 64 : 32;
   static constexpr int TURN_ROW = TURN_COLS * 4 + 16;  // + 16: rows start in different banks
   static constexpr int TURN_BYTES = WAVES * 32 * TURN_ROW;
-  static constexpr int MAIN_BYTES = STAGES * STAGE_BYTES;
+  static constexpr int MAIN_BYTES = STAGES * (A_BYTES + B_BYTES);
   static constexpr int LDS_BYTES = MAIN_BYTES > TURN_BYTES ? MAIN_BYTES : TURN_BYTES;
 };
 
-// acc = the products of K tiles [kt0, kt0 + kts) of block (tm, tn).
-template <int BM, int BN, int BK, int WAVES, int STAGES, bool BT, bool NTB, bool SEG3>
+// Loaders of one K tile of 64: each wave load brings 1 KiB, lane l's 16 bytes
+// landing at 16 l of its piece, so the lane fetches what the swizzle puts
+// there.  Load j covers the rows j * WAVES loads further on; the swizzle
+// repeats over that (every second load, N contiguous), so a lane keeps one
+// or two offsets, and the rest rides in the scalar base address.
+// Reads past `bytes` give 0.
+//
+// The descriptor must come out of scalar instructions: the load is inline
+// assembly, so the compiler does not see that it reads scalar registers and
+// leaves out the wait states that a vector instruction's write to one needs
+// (a saturating subtraction is such an instruction; the empty asm keeps the
+// minimum and the difference from becoming one).
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t epi_rsrc(const uint16_t* p, uint32_t bytes, uint32_t off) {
+  off = __builtin_amdgcn_readfirstlane(off);
+  uint32_t at = off < bytes ? off : bytes;
+  asm("" : "+s"(at));
+  return make_rsrc((const char*)p + at, bytes - at);
+}
+// ROWS rows of 64 consecutive k (K contiguous).
+template <int ROWS, int WAVES>
+struct EpiKLoad {
+  static constexpr int LOADS = ROWS / 8 / WAVES;
+  static_assert(LOADS >= 1 && ROWS % (8 * WAVES) == 0 && WAVES % 2 == 0, "whole loads, the same swizzle in each");
+  uint32_t voff, voff_tail, first, step;
+  int lds;
+  __device__ __forceinline__ void init(int wave, int lane, int row0, int ld, int k_last) {
+    const int r = wave * 8 + (lane >> 3), q = (lane & 7) ^ k_swz<64>(r);
+    voff = ((uint32_t)r * (uint32_t)ld + (uint32_t)(8 * q)) * 2u;
+    voff_tail = 8 * q < k_last ? voff : 0xFFFFFFF0u;
+    first = (uint32_t)row0 * (uint32_t)ld * 2u;
+    step = (uint32_t)(WAVES * 8) * (uint32_t)ld * 2u;
+    lds = wave * 1024;
+  }
+  template <bool NT>
+  __device__ __forceinline__ void issue(int j, const uint16_t* p, uint32_t bytes, uint32_t tile, char* panel,
+                                        bool tail) const {
+    lds_dma16<NT>(epi_rsrc(p, bytes, first + (uint32_t)j * step + tile), panel + lds + j * WAVES * 1024,
+                  tail ? voff_tail : voff);
+  }
+};
+// 64 rows of COLS consecutive n (N contiguous).
+template <int COLS, int WAVES>
+struct EpiNLoad {
+  static constexpr int LOADS = COLS / 8 / WAVES, ROWB = COLS * 2, RPL = 1024 / ROWB;
+  static_assert(LOADS >= 1 && COLS % (8 * WAVES) == 0 && 2 * WAVES * RPL % 16 == 0, "whole loads, two swizzles");
+  uint32_t voff[2], first, step;
+  int lds;
+  __device__ __forceinline__ void init(int wave, int lane, int col0, int ld, int) {
+    const int r = wave * RPL + lane / (COLS / 8), slot = lane % (COLS / 8);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      voff[i] = ((uint32_t)r * (uint32_t)ld + (uint32_t)(8 * (slot ^ mn_swz<ROWB>(r + i * WAVES * RPL)))) * 2u;
+    first = (uint32_t)col0 * 2u;
+    step = (uint32_t)(WAVES * RPL) * (uint32_t)ld * 2u;
+    lds = wave * 1024;
+  }
+  template <bool NT>
+  __device__ __forceinline__ void issue(int j, const uint16_t* p, uint32_t bytes, uint32_t tile, char* panel, bool) const {
+    lds_dma16<NT>(epi_rsrc(p, bytes, first + (uint32_t)j * step + tile), panel + lds + j * WAVES * 1024, voff[j & 1]);
+  }
+};
+
+// acc = the products of K tiles [kt0, kt0 + kts) of block (tm, tn).  Lane l,
+// register r of acc[i][j]: row 16 i + l % 16, column 16 j + 4 (l / 16) + r of
+// the wave's part.
+template <int BM, int BN, int BK, int WAVES, int STAGES, bool BT, bool NTB, bool SEG3, int TM, int TN>
 __device__ __forceinline__ void epi_main(const EpiMM& p, const uint16_t* a, const uint16_t* b, char* smem, int tmi,
-                                         int tni, int kt0, int kts,
-                                         f32x16_t (&acc)[WaveGrid<BM, BN, WAVES>::TM][WaveGrid<BM, BN, WAVES>::TN]) {
+                                         int tni, int kt0, int kts, f32x4_t (&acc)[TM][TN]) {
   using C = EpiCfg<BM, BN, BK, WAVES, STAGES>;
   using G = typename C::G;
-  static_assert(G::ok && BK % 32 == 0 && STAGES >= 2 && STAGES <= 4, "tile config");
+  static_assert(G::ok && BK == 64 && STAGES >= 2 && STAGES <= 4, "tile config");
+  static_assert(TM == C::TM && TN == C::TN, "accumulators of the wave's part");
   static_assert(C::LDS_BYTES <= kLdsBytesMax, "LDS over 160 KiB");
-  constexpr int TM = G::TM, TN = G::TN, KS = BK / 16, NF = TM + TN;
-  using LA = KPanelLoader<BK, BM, WAVES>;
-  using LB = std::conditional_t<BT, KPanelLoader<BK, BN, WAVES>, PanelLoader<BK, BN, WAVES>>;
-  constexpr int LPT = LA::LOADS_PER_TILE + LB::LOADS_PER_TILE;
-  static_assert(LA::EVEN && LB::EVEN, "every wave issues the same number of loads (vm_wait counts them)");
+  constexpr int KS = BK / 32, NF = TM + TN, NM = TM * TN;
+  using LA = EpiKLoad<BM, WAVES>;
+  using LB = std::conditional_t<BT, EpiKLoad<BN, WAVES>, EpiNLoad<BN, WAVES>>;
+  constexpr int LPT = LA::LOADS + LB::LOADS;  // of every wave: vm_wait counts them
   static_assert((STAGES - 1) * LPT < 64, "loads in flight exceed the 6-bit vmcnt");
 
   const int tid = (int)threadIdx.x, lane = tid & 63;
@@ -78,53 +146,62 @@ __device__ __forceinline__ void epi_main(const EpiMM& p, const uint16_t* a, cons
   const int k_last = p.K - (KT1 - 1) * BK;
   LA la;
   LB lb;
-  la.init(wave, lane, m0, p.lda, k_last, p.a_bytes);
-  if constexpr (BT) lb.init(wave, lane, n0, p.ldb, k_last, p.b_bytes);
-  else lb.init(wave, lane, n0, p.ldb);
-  using FB = TrFrag<BN, TN, BK>;
-  FB fb;
-  if constexpr (!BT) fb.init(lane, wn0);
-  // K-contiguous operands: lane l reads row l%32 of a fragment, K chunk
-  // 2*kk + l/32 of the step, at its k_swz slot.
-  const int arow = (wm0 + (lane & 31)) * (BK * 2), brow = (wn0 + (lane & 31)) * (BK * 2);
-  int akoff[KS], bkoff[KS];
+  la.init(wave, lane, m0, p.lda, k_last);
+  lb.init(wave, lane, n0, p.ldb, k_last);
+  // K-contiguous operands: lane l reads row l % 16 of a fragment, K chunk
+  // 4 kk + l / 16 of the tile, at its k_swz slot (the same for every
+  // fragment: the swizzle repeats every 16 rows).
+  const int row = lane & 15, chunk = lane >> 4;
+  const int arow = (wm0 + row) * (BK * 2), brow = C::B_OFF + (wn0 + row) * (BK * 2);
+  int koff[KS];
 #pragma unroll
-  for (int kk = 0; kk < KS; ++kk) {
-    akoff[kk] = 16 * ((2 * kk + (lane >> 5)) ^ k_swz<BK>(wm0 + (lane & 31)));
-    bkoff[kk] = 16 * ((2 * kk + (lane >> 5)) ^ k_swz<BK>(wn0 + (lane & 31)));
+  for (int kk = 0; kk < KS; ++kk) koff[kk] = 16 * ((4 * kk + chunk) ^ k_swz<BK>(row));
+  // N-contiguous B: 16 lanes read 4 rows of 16 columns and each gets one
+  // column of them; lanes 16 g .. 16 g + 15 take K rows 8 g .. 8 g + 7 in two
+  // reads.
+  constexpr int ROWB = BN * 2;
+  int boff[TN];
+  if constexpr (!BT) {
+    const int krow = 8 * chunk + (row >> 2);
+#pragma unroll
+    for (int t = 0; t < TN; ++t) {
+      const int col = wn0 + 16 * t + 4 * (row & 3);
+      boff[t] = C::B_OFF + krow * ROWB + 16 * ((col >> 3) ^ mn_swz<ROWB>(krow)) + (col & 7) * 2;
+    }
   }
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = f32x16_t{};
+    for (int j = 0; j < TN; ++j) acc[i][j] = f32x4_t{};
 
   bf16x8_t af[2][TM], bf[2][TN];
+  // Operand f of step kk, in the order the MFMAs (row-major) take them: A0,
+  // B0 .. B(TN-1), A1 .. A(TM-1).
   auto read_frag = [&](int stage, int kk, int buf, int f) __attribute__((always_inline)) {
-    const int abase = stage * C::STAGE_BYTES, bbase = abase + C::A_BYTES;
+    const int abase = stage * C::A_BYTES, bbase = stage * C::B_BYTES;
     if (f == 0 || f > TN) {
       const int t = f == 0 ? 0 : f - TN;
       af[buf][t] = __builtin_bit_cast(
-          bf16x8_t, *(MI_LDS u32x4_t*)((MI_LDS char*)smem + abase + arow + t * 32 * (BK * 2) + akoff[kk]));
+          bf16x8_t, *(MI_LDS u32x4_t*)((MI_LDS char*)smem + abase + arow + t * 16 * (BK * 2) + koff[kk]));
     } else {
       const int t = f - 1;
       if constexpr (BT)
         bf[buf][t] = __builtin_bit_cast(
-            bf16x8_t, *(MI_LDS u32x4_t*)((MI_LDS char*)smem + bbase + brow + t * 32 * (BK * 2) + bkoff[kk]));
+            bf16x8_t, *(MI_LDS u32x4_t*)((MI_LDS char*)smem + bbase + brow + t * 16 * (BK * 2) + koff[kk]));
       else
-        bf[buf][t] = read_tr_frag(smem, bbase + (kk * 16) * FB::ROWB + fb.off[t],
-                                  bbase + (kk * 16 + 4) * FB::ROWB + fb.off[t]);
+        bf[buf][t] = read_tr_frag(smem, bbase + (kk * 32) * ROWB + boff[t], bbase + (kk * 32 + 4) * ROWB + boff[t]);
     }
   };
   auto read_frags = [&](int stage, int kk, int buf) __attribute__((always_inline)) {
 #pragma unroll
     for (int f = 0; f < NF; ++f) read_frag(stage, kk, buf, f);
   };
-  auto mfmas = [&](int buf) __attribute__((always_inline)) {
+  // MFMAs [lo, hi) of the fragments in `buf`, row-major.
+  auto mfmas = [&](int buf, int lo, int hi) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-      for (int j = 0; j < TN; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bf[buf][j], af[buf][i], acc[i][j], 0, 0, 0);
+    for (int x = lo; x < hi; ++x)
+      acc[x / TN][x % TN] =
+          __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf[buf][x % TN], af[buf][x / TN], acc[x / TN][x % TN], 0, 0, 0);
   };
   constexpr int READS = TM + (BT ? TN : 2 * TN);  // LDS reads of one step
   // Load q (< LPT) of K tile t of this block's range into `stage`.
@@ -137,18 +214,13 @@ __device__ __forceinline__ void epi_main(const EpiMM& p, const uint16_t* a, cons
       r = kt - (hi_a ? 2 * KT1 : hi_b ? KT1 : 0);
     }
     const bool tail = !SEG3 && kt == KT1 - 1;
-    if (q < LA::LOADS_PER_TILE) {
+    if (q < LA::LOADS) {
       const uint32_t off = (uint32_t)r * (uint32_t)(BK * 2) + (SEG3 && hi_a ? p.plane_a : 0u);
-      la.issue_at(q, make_rsrc_from(a, p.a_bytes, off), smem, stage * C::STAGE_BYTES, tail);
+      la.template issue<false>(q, a, p.a_bytes, off, smem + stage * C::A_BYTES, tail);
     } else {
       const uint32_t off = (uint32_t)r * (BT ? (uint32_t)(BK * 2) : (uint32_t)BK * (uint32_t)p.ldb * 2u) +
                            (SEG3 && hi_b ? p.plane_b : 0u);
-      if constexpr (BT)
-        lb.template issue_at<NTB>(q - LA::LOADS_PER_TILE, make_rsrc_from(b, p.b_bytes, off), smem,
-                                  stage * C::STAGE_BYTES + C::A_BYTES, tail);
-      else
-        lb.template issue_at<NTB>(q - LA::LOADS_PER_TILE, make_rsrc_from(b, p.b_bytes, off), smem,
-                                  stage * C::STAGE_BYTES + C::A_BYTES);
+      lb.template issue<NTB>(q - LA::LOADS, b, p.b_bytes, off, smem + C::B_OFF + stage * C::B_BYTES, tail);
     }
   };
   // Tiles past the range are the last one again (into a buffer that nobody
@@ -163,86 +235,159 @@ __device__ __forceinline__ void epi_main(const EpiMM& p, const uint16_t* a, cons
   __syncthreads();
   read_frags(0, 0, 0);
 
-  // At the last step of tile t the wave waits for its loads of tile t+1,
-  // meets the workgroup (tile t+1 is whole, tile t's buffer free), reads tile
-  // t+1's first operands and requests tile t+STAGES.
-  auto tile = [&](int t, auto cur_c) __attribute__((always_inline)) {
-    constexpr int cur = decltype(cur_c)::value, nxt = (cur + 1) % STAGES;
+  if constexpr (STAGES == 2) {
+    // Two stages.  A stage is read within half a tile (both steps' fragments
+    // are in registers from the middle of step 0 on), so the loads that
+    // refill it are in flight for 1.4 tiles rather than 1:
+    //   step 0: fragments of step 1 read in its first half; three quarters
+    //           in, every wave has them, the stage is free and the loads of
+    //           tile t+2 go out behind it, up to the middle of step 1;
+    //   step 1: in its middle tile t+1 has landed, and the fragments of its
+    //           step 0 are read.
+    constexpr int HM = NM / 2, QM = NM / 4, SLOTS = NM / 2;
+    auto tile = [&](int t, auto cur_c) __attribute__((always_inline)) {
+      constexpr int cur = decltype(cur_c)::value;
+      read_frags(cur, 1, 1);
+      mfmas(0, 0, HM);
+      interleave_mfma_ds<HM, READS>();
+      mfmas(0, HM, HM + QM);
+      __builtin_amdgcn_sched_barrier(0);
+      __syncthreads();
+      const int t_new = clamp(t + 2);
+      static_for<SLOTS>([&](auto x_c) __attribute__((always_inline)) {
+        constexpr int x = decltype(x_c)::value;
 #pragma unroll
-    for (int kk = 0; kk + 1 < KS; ++kk) {
-      read_frags(cur, kk + 1, (kk + 1) & 1);
-      mfmas(kk & 1);
-      interleave_mfma_ds<TM * TN, READS>();
-    }
-    vm_wait<(STAGES - 2) * LPT>();
-    __syncthreads();
-    const int t_new = clamp(t + STAGES);
+        for (int q = x * LPT / SLOTS; q < (x + 1) * LPT / SLOTS; ++q) issue_one(q, t_new, cur);
+        if constexpr (x < NM - HM - QM) mfmas(0, HM + QM + x, HM + QM + x + 1);
+        else mfmas(1, x - (NM - HM - QM), x - (NM - HM - QM) + 1);
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      constexpr int DONE = SLOTS - (NM - HM - QM);  // MFMAs of step 1 so far
+      mfmas(1, DONE, HM);
+      __builtin_amdgcn_sched_barrier(0);
+      vm_wait<LPT>();
+      __syncthreads();
+      read_frags(cur ^ 1, 0, 0);
+      mfmas(1, HM, NM);
+      interleave_mfma_ds<NM - HM, READS>();
+    };
+    int t0 = 0;
+    for (; t0 + 2 < kts; t0 += 2)
+      static_for<2>([&](auto s_c) __attribute__((always_inline)) { tile(t0 + s_c(), s_c); });
+    if (t0 + 1 < kts) tile(t0, std::integral_constant<int, 0>{});
+    read_frags((kts - 1) & 1, 1, 1);
+    mfmas(0, 0, NM);
+    mfmas(1, 0, NM);
+  } else {
+    // At the last step of tile t the wave waits for its loads of tile t+1,
+    // meets the workgroup (tile t+1 is whole, tile t's buffer free), reads
+    // tile t+1's first operands and requests tile t+STAGES.
+    auto tile = [&](int t, auto cur_c) __attribute__((always_inline)) {
+      constexpr int cur = decltype(cur_c)::value, nxt = (cur + 1) % STAGES;
+      read_frags(cur, 1, 1);
+      mfmas(0, 0, NM);
+      interleave_mfma_ds<NM, READS>();
+      vm_wait<(STAGES - 2) * LPT>();
+      __syncthreads();
+      const int t_new = clamp(t + STAGES);
 #pragma unroll
-    for (int f = 0; f < NF; ++f) {
-      read_frag(nxt, 0, 0, f);
+      for (int f = 0; f < NF; ++f) {
+        read_frag(nxt, 0, 0, f);
 #pragma unroll
-      for (int q = f * LPT / NF; q < (f + 1) * LPT / NF; ++q) issue_one(q, t_new, cur);
-    }
-    mfmas((KS - 1) & 1);
-    interleave_mfma_ds<TM * TN, READS>();
-  };
-  int t0 = 0;
-  for (; t0 + STAGES < kts; t0 += STAGES)
-    static_for<STAGES>([&](auto s_c) __attribute__((always_inline)) { tile(t0 + s_c(), s_c); });
-  static_while<STAGES>([&](auto s_c) __attribute__((always_inline)) {
-    if (t0 + s_c() + 1 >= kts) return false;
-    tile(t0 + s_c(), s_c);
-    return true;
-  });
-  const int cur = (kts - 1) % STAGES;
-#pragma unroll
-  for (int kk = 0; kk < KS; ++kk) {
-    if (kk + 1 < KS) read_frags(cur, kk + 1, (kk + 1) & 1);
-    mfmas(kk & 1);
-    interleave_mfma_ds<TM * TN, READS>();
+        for (int q = f * LPT / NF; q < (f + 1) * LPT / NF; ++q) issue_one(q, t_new, cur);
+      }
+      mfmas(1, 0, NM);
+      interleave_mfma_ds<NM, READS>();
+    };
+    int t0 = 0;
+    for (; t0 + STAGES < kts; t0 += STAGES)
+      static_for<STAGES>([&](auto s_c) __attribute__((always_inline)) { tile(t0 + s_c(), s_c); });
+    static_while<STAGES>([&](auto s_c) __attribute__((always_inline)) {
+      if (t0 + s_c() + 1 >= kts) return false;
+      tile(t0 + s_c(), s_c);
+      return true;
+    });
+    read_frags((kts - 1) % STAGES, 1, 1);
+    mfmas(0, 0, NM);
+    mfmas(1, 0, NM);
   }
   wait_vmem();
   __syncthreads();  // the epilogue reuses the panel buffers
 }
 
-// Hands each lane 8 consecutive columns of the wave's accumulators at a time:
-// f.columns(n) once per column group, f.fetch(it, m, n) before a turn and
-// f.apply(it, m, n, v) after it, it < F::ROWS (rows a lane has per turn).
+// Hands each lane 8 consecutive columns of the wave's accumulators at a time.
+// For each group of columns f.columns(n); then for each turn of 32 rows
+// f.fetch(it, r, n) one turn ahead, f.arrived() and f.apply(it, r, n, v), it <
+// IT rows a lane has in a turn, r counted from the block's first row.
+//
+// Both loops are run-time ones: the code after a turn stands once, and only
+// the writes that name accumulator registers are there for each slice
+// (unrolled, the epilogue of a 128x128 wave tile is 12000 instructions, and
+// where the compiler leaves the loop to run time by itself it keeps the
+// accumulators in memory).  Loads and stores share one counter and are
+// counted off in order, so a wait for a load waits for every store before it:
+// the rows of turn s+1 are requested before the stores of turn s, and f has
+// no branch around a load or store, which would make the compiler wait for
+// all of them.
 template <int TM, int TN, int ROWB, class F>
-__device__ __forceinline__ void epi_rows(const f32x16_t (&acc)[TM][TN], char* smem, int wave, int lane, int row0,
+__device__ __forceinline__ void epi_rows(const f32x4_t (&acc)[TM][TN], char* smem, int wave, int lane, int row0,
                                          int col0, F& f) {
-  constexpr int TW = TN >= 2 ? 2 : 1, LPR = 4 * TW, RPI = 64 / LPR, IT = 32 / RPI;
-  static_assert(TN % TW == 0 && ROWB == TW * 128 + 16 && IT <= 4, "turn layout");
+  constexpr int TW = TN >= 4 ? 2 : 1, LPR = 4 * TW, RPI = 64 / LPR, IT = 32 / RPI, NP = TN / (2 * TW), MT = TM / 2;
+  static_assert(TN % (2 * TW) == 0 && TM % 2 == 0 && ROWB == TW * 128 + 16 && IT <= 4, "turn layout");
   MI_LDS char* slot = (MI_LDS char*)smem + wave * (32 * ROWB);
+  const int n0 = col0 + 8 * (lane % LPR), r0 = row0 + lane / LPR;
 #pragma unroll
-  for (int np = 0; np < TN / TW; ++np) {
-    const int n = col0 + np * TW * 32 + 8 * (lane % LPR);
+  for (int it = 0; it < IT; ++it) f.fetch(it, r0 + it * RPI, n0);
+#pragma unroll 1
+  for (int np = 0; np < NP; ++np) {
+    const int n = n0 + np * (TW * 32);
     f.columns(n);
+#pragma unroll 1
+    for (int mt = 0; mt < MT; ++mt) {
+      const int s = np * MT + mt;
+      f.arrived();
+      const int r_next = r0 + (mt + 1 < MT ? mt + 1 : 0) * 32, n_next = n + (mt + 1 < MT ? 0 : TW * 32);
 #pragma unroll
-    for (int mt = 0; mt < TM; ++mt) {
-      const int m = row0 + mt * 32 + lane / LPR;
+      for (int it = 0; it < IT; ++it) f.fetch(it, r_next + it * RPI, n_next);
+      static_for<NP * MT>([&](auto k_c) __attribute__((always_inline)) {
+        constexpr int k = decltype(k_c)::value;
+        if (s != k) return;
 #pragma unroll
-      for (int it = 0; it < IT; ++it) f.fetch(it, m + it * RPI, n);
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int h = 0; h < TW; ++h)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const f32x16_t& x = acc[mt][np * TW + h];
-          const f32x4_t v = {x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]};
-          *(MI_LDS f32x4_t*)(slot + (lane & 31) * ROWB + h * 128 + 32 * j + 16 * (lane >> 5)) = v;
-        }
+          for (int j = 0; j < 2 * TW; ++j)
+            *(MI_LDS f32x4_t*)(slot + (16 * i + (lane & 15)) * ROWB + 64 * j + 16 * (lane >> 4)) =
+                acc[k % MT * 2 + i][k / MT * 2 * TW + j];
+      });
       wave_lds_turn();
 #pragma unroll
       for (int it = 0; it < IT; ++it) {
         MI_LDS char* at = slot + (it * RPI + lane / LPR) * ROWB + 32 * (lane % LPR);
         const f32x4_t lo = *(MI_LDS f32x4_t*)at, hi = *(MI_LDS f32x4_t*)(at + 16);
         float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-        f.apply(it, m + it * RPI, n, v);
+        f.apply(it, r0 + mt * 32 + it * RPI, n, v);
       }
       wave_lds_turn();
     }
   }
 }
+
+// 16-byte accesses to rows of a tensor, from the block's first row on:
+// past `bytes` a load gives 0 and a store does nothing, without a branch.  A
+// tensor that is not there has no bytes.
+struct EpiRows {
+  __amdgpu_buffer_rsrc_t rs;
+  __device__ __forceinline__ void init(const void* p, long long first, long long count) {
+    rs = make_rsrc(p ? (const char*)p + first : nullptr, p ? (uint32_t)count : 0u);
+  }
+  __device__ __forceinline__ u32x4_t load(uint32_t off) const {
+    return __builtin_amdgcn_raw_buffer_load_b128(rs, (int)off, 0, 0);
+  }
+  __device__ __forceinline__ void store(uint32_t off, u32x4_t v) const {
+    __builtin_amdgcn_raw_buffer_store_b128(v, rs, (int)off, 0, 0);
+  }
+};
+constexpr uint32_t kEpiNowhere = 0xFFFFFFF0u;  // past every EpiRows
 
 __device__ __forceinline__ u32x4_t pack8(const float (&v)[8]) {
   return u32x4_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
@@ -265,7 +410,7 @@ struct EpiOut {
   bool bias_f32, vec;
 
   float b[8];
-  u32x4_t res[4];
+  int m0;  // the block's first row
 
   __device__ __forceinline__ float bias_at(int n) const {
     return bias_f32 ? ((const float*)bias)[n] : bf16lo((uint32_t)((const uint16_t*)bias)[n]);
@@ -291,10 +436,10 @@ struct EpiOut {
         if (n + i < N) b[i] = bias_at(n + i);
     }
   }
-  __device__ __forceinline__ void fetch(int it, int m, int n) {
-    if (residual && vec && m < M && n < N) res[it] = *(const u32x4_t*)(residual + (size_t)m * (size_t)N + n);
-  }
-  __device__ __forceinline__ void apply(int it, int m, int n, float (&v)[8]) {
+  __device__ __forceinline__ void fetch(int, int, int) {}
+  __device__ __forceinline__ void arrived() {}
+  __device__ __forceinline__ void apply(int, int r, int n, float (&v)[8]) {
+    const int m = m0 + r;
     if (m >= M || n >= N) return;
     const size_t at = (size_t)m * (size_t)N + n;
 #pragma unroll
@@ -314,10 +459,10 @@ struct EpiOut {
     });
     if (vec) {
       if (residual) {
-        float r[8];
-        unpack8(res[it], r);
+        float x[8];
+        unpack8(*(const u32x4_t*)(residual + at), x);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] += r[i];
+        for (int i = 0; i < 8; ++i) v[i] += x[i];
       }
       *(u32x4_t*)(out + at) = pack8(v);
     } else {
@@ -331,6 +476,60 @@ struct EpiOut {
   }
 };
 
+// EpiOut's function where `vec` holds, without a branch around a load or
+// store.
+struct EpiVec {
+  EpiRows out, pre, residual, bias16, bias32;
+  int N, act;
+  float b[8];
+  u32x4_t next[4], res[4];
+
+  __device__ __forceinline__ void init(const EpiOut& e, int m0, int bm) {
+    const long long first = (long long)m0 * e.N * 2, rows = e.M - m0 < bm ? e.M - m0 : bm;
+    out.init(e.out, first, rows * e.N * 2);
+    pre.init(e.pre, first, rows * e.N * 2);
+    residual.init(e.residual, first, rows * e.N * 2);
+    bias16.init(e.bias_f32 ? nullptr : e.bias, 0, (long long)e.N * 2);
+    bias32.init(e.bias_f32 ? e.bias : nullptr, 0, (long long)e.N * 4);
+    N = e.N;
+    act = e.act;
+  }
+  __device__ __forceinline__ uint32_t at(int r, int n) const {
+    return n < N ? ((uint32_t)r * (uint32_t)N + (uint32_t)n) * 2u : kEpiNowhere;
+  }
+  __device__ __forceinline__ void columns(int n) {
+    const u32x4_t h = bias16.load(n < N ? (uint32_t)n * 2u : kEpiNowhere);
+    const u32x4_t f0 = bias32.load(n < N ? (uint32_t)n * 4u : kEpiNowhere);
+    const u32x4_t f1 = bias32.load(n < N ? (uint32_t)n * 4u + 16u : kEpiNowhere);
+    unpack8(h, b);  // one of the two is 0
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      b[i] += __builtin_bit_cast(float, (uint32_t)f0[i]);
+      b[4 + i] += __builtin_bit_cast(float, (uint32_t)f1[i]);
+    }
+  }
+  __device__ __forceinline__ void fetch(int it, int r, int n) { next[it] = residual.load(at(r, n)); }
+  __device__ __forceinline__ void arrived() {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) res[i] = next[i];
+  }
+  __device__ __forceinline__ void apply(int it, int r, int n, float (&v)[8]) {
+    const uint32_t off = at(r, n);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += b[i];
+    pre.store(off, pack8(v));
+    with_act(act, [&](auto a_c) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = act_value<decltype(a_c)::value>(v[i]);
+    });
+    float x[8];
+    unpack8(res[it], x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += x[i];
+    out.store(off, pack8(v));
+  }
+};
+
 // out = act(A . B + bias) + residual, one workgroup per block.
 template <int BM, int BN, int BK, int WAVES, int STAGES, bool BT, bool NTB>
 __global__ __launch_bounds__(WAVES * 64) void mm_epi_kernel(const EpiMM p, EpiOut e) {
@@ -339,12 +538,38 @@ __global__ __launch_bounds__(WAVES * 64) void mm_epi_kernel(const EpiMM p, EpiOu
   __shared__ __attribute__((aligned(1024))) char smem[C::LDS_BYTES];
   int tm, tn;
   tile_coords((p.M + BM - 1) / BM, (p.N + BN - 1) / BN, p.group_m, tm, tn);
-  f32x16_t acc[G::TM][G::TN];
+  f32x4_t acc[C::TM][C::TN];
   epi_main<BM, BN, BK, WAVES, STAGES, BT, NTB, false>(p, p.a, p.b, smem, tm, tn, 0, (p.K + BK - 1) / BK, acc);
   const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  epi_rows<G::TM, G::TN, C::TURN_ROW>(acc, smem, wave, lane, tm * BM + (wave / G::WN) * G::WTM,
-                                      tn * BN + (wave % G::WN) * G::WTN, e);
+  const int row0 = (wave / G::WN) * G::WTM, col0 = tn * BN + (wave % G::WN) * G::WTN;
+  if (e.vec) {
+    EpiVec v;
+    v.init(e, tm * BM, BM);
+    epi_rows<C::TM, C::TN, C::TURN_ROW>(acc, smem, wave, lane, row0, col0, v);
+  } else {
+    e.m0 = tm * BM;
+    epi_rows<C::TM, C::TN, C::TURN_ROW>(acc, smem, wave, lane, row0, col0, e);
+  }
 }
+
+// fp32 products of one part of K, rows ldw apart.
+struct EpiPart {
+  EpiRows ws;
+  int ldw;
+  __device__ __forceinline__ void init(const float* p, int M, int ld, int m0, int bm) {
+    const long long rows = M - m0 < bm ? M - m0 : bm;
+    ws.init(p, (long long)m0 * ld * 4, rows * ld * 4);
+    ldw = ld;
+  }
+  __device__ __forceinline__ void columns(int) {}
+  __device__ __forceinline__ void fetch(int, int, int) {}
+  __device__ __forceinline__ void arrived() {}
+  __device__ __forceinline__ void apply(int, int r, int n, float (&v)[8]) {
+    const uint32_t off = n < ldw ? ((uint32_t)r * (uint32_t)ldw + (uint32_t)n) * 4u : kEpiNowhere;
+    ws.store(off, __builtin_bit_cast(u32x4_t, f32x4_t{v[0], v[1], v[2], v[3]}));
+    ws.store(n < ldw ? off + 16u : kEpiNowhere, __builtin_bit_cast(u32x4_t, f32x4_t{v[4], v[5], v[6], v[7]}));
+  }
+};
 
 // The same over one of p.parts ranges of K tiles: fp32 products to
 // ws[part][M][ldw], ldw = N rounded up to 8; epi_sum_kernel adds them.
@@ -356,13 +581,13 @@ __global__ __launch_bounds__(WAVES * 64) void mm_epi_split_kernel(const EpiMM p,
   int tm, tn, part;
   tile_coords_split((p.M + BM - 1) / BM, (p.N + BN - 1) / BN, p.group_m, p.parts, tm, tn, part);
   const int KT = (p.K + BK - 1) / BK, each = (KT + p.parts - 1) / p.parts, kt0 = part * each;
-  f32x16_t acc[G::TM][G::TN];
+  f32x4_t acc[C::TM][C::TN];
   epi_main<BM, BN, BK, WAVES, STAGES, BT, NTB, false>(p, p.a, p.b, smem, tm, tn, kt0, KT - kt0 < each ? KT - kt0 : each,
                                                       acc);
   const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  constexpr int ROWS = partial_rows(WAVES, C::LDS_BYTES);
-  store_partial<G::TM, G::TN, ROWS>(acc, ws + (size_t)part * (size_t)p.M * (size_t)ldw, smem, wave, lane, p.M, ldw,
-                                    tm * BM + (wave / G::WN) * G::WTM, tn * BN + (wave % G::WN) * G::WTN);
+  EpiPart f;
+  f.init(ws + (size_t)part * (size_t)p.M * (size_t)ldw, p.M, ldw, tm * BM, BM);
+  epi_rows<C::TM, C::TN, C::TURN_ROW>(acc, smem, wave, lane, (wave / G::WN) * G::WTM, tn * BN + (wave % G::WN) * G::WTN, f);
 }
 
 }  // namespace mi

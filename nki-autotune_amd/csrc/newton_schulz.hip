@@ -219,14 +219,14 @@ int mi_newton_schulz(const mi_newton_schulz_args* args, void* workspace, unsigne
   const bool direct = !q.turn && n == lp && (uintptr_t)args->out % 16 == 0;  // the last product stores out itself
   for (int k = 0; k < args->steps; ++k) {
     const EpiMM gram = {x, x, xb, xb, s, sp, lp, 2 * lp, 2 * lp, 8, 1, (uint32_t)lp * 2, (uint32_t)lp * 2, xz, xz};
-    const NsOut to_a = {nullptr, A, nullptr, s, sp, 2 * sp, 1.0f, 0.0f, 0, az};
+    const NsOut to_a = {nullptr, A, nullptr, s, sp, 2 * sp, 1.0f, 0.0f, 0, az, 0};
     if ((rc = product<true>(gram, to_a, batch, st)) != MI_OK) return rc;
     const EpiMM square = {A, A, ab, ab, s, sp, sp, 2 * sp, 2 * sp, 8, 1, (uint32_t)sp * 2, (uint32_t)sp * 2, az, az};
-    const NsOut to_b = {A, B, nullptr, s, sp, 2 * sp, args->c, args->b, az, az};
+    const NsOut to_b = {A, B, nullptr, s, sp, 2 * sp, args->c, args->b, az, az, 0};
     if ((rc = product<true>(square, to_b, batch, st)) != MI_OK) return rc;
     const EpiMM update = {B, x, ab, xb, s, lp, sp, 2 * sp, 2 * lp, 8, 1, (uint32_t)sp * 2, (uint32_t)lp * 2, az, xz};
     const bool last = direct && k + 1 == args->steps;
-    const NsOut to_x = {x, next, last ? (uint16_t*)args->out : nullptr, s, lp, 2 * lp, 1.0f, args->a, xz, last ? per : xz};
+    const NsOut to_x = {x, last ? nullptr : next, last ? (uint16_t*)args->out : nullptr, s, lp, 2 * lp, 1.0f, args->a, xz, xz, per};
     if ((rc = product<false>(update, to_x, batch, st)) != MI_OK) return rc;
     uint16_t* t = x;
     x = next;
