@@ -180,20 +180,42 @@ const EpiEntry* find(bool bt, const mi_tile_cfg& c) {
   return nullptr;
 }
 
-// The library's choice of a config for a product of these sizes.
+// The library's choice of a config for a product of these sizes: the least
+// estimated time (mi_epi_table.hpp) over the configs and part counts.  The
+// busiest unit's blocks run one after the other, or share it; no product is
+// faster than its bytes at 5.4 TB/s; parts cost a second launch and their
+// fp32 products written and read.
 mi_tile_cfg pick(int M, int N, int K, bool bt) {
-  (void)bt;
-  mi_tile_cfg c = {256, 256, 64, 8, 2, 1, 8, 0};
-  const auto tiles = [&](int bm, int bn) { return (long long)((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
-  if (M <= 64) c = {M <= 32 ? 32 : 64, 128, 64, 4, 4, 1, 8, 1};
-  else if (tiles(256, 256) < 200) c = tiles(128, 128) >= 200 ? mi_tile_cfg{128, 128, 64, 4, 2, 1, 8, 0} : mi_tile_cfg{64, 64, 64, 4, 4, 1, 8, 0};
-  const long long t = tiles(c.block_m, c.block_n);
+  int n = 0;
+  const EpiEntry* t = table(bt, &n);
+  const int cus = mi::capi::device_cus();
+  const double mem = 2.0 * ((double)N * K + (double)M * K + (double)M * N) / 5.4e6;
   const int kt = (K + 63) / 64;
-  int parts = 1;
-  while (parts < kMaxSplit && t * parts * 2 <= 512 && kt / (parts * 2) >= 8) parts *= 2;
-  const int each = (kt + parts - 1) / parts;
-  c.split_k = each > 0 ? (kt + each - 1) / each : 1;
-  return c;
+  mi_tile_cfg best = t[0].cfg;
+  double least = 1e30;
+  for (int i = 0; i < n; ++i) {
+    const EpiEntry& e = t[i];
+    const long long tiles =
+        (long long)((M + e.cfg.block_m - 1) / e.cfg.block_m) * ((N + e.cfg.block_n - 1) / e.cfg.block_n);
+    for (const int parts : {1, 2, 3, 4, 6, 8, 12, 16}) {
+      const int each = (kt + parts - 1) / parts;
+      // Parts of at least three K tiles, none empty, in at most four blocks a unit.
+      if (parts > 1 && (kt / parts < 3 || (parts - 1) * each >= kt || tiles * parts > 4ll * cus ||
+                        (double)parts * M * N * 4.0 > (double)mi::capi::kMaxWorkspace))
+        break;
+      const long long blocks = (tiles * parts + cus - 1) / cus, rounds = (blocks + e.per_cu - 1) / e.per_cu;
+      const double in_line = (double)blocks * e.shared * each, alone = (double)rounds * e.alone * each;
+      double us = (in_line > alone ? in_line : alone) + (double)rounds * e.ends;
+      if (us < mem) us = mem;
+      if (parts > 1) us += 3.0 + (double)parts * M * N * 2e-6;
+      if (us < least) {
+        least = us;
+        best = e.cfg;
+        best.split_k = parts;
+      }
+    }
+  }
+  return best;
 }
 
 // One product A . B or A . B^T with an epilogue, operands already in rows of
@@ -228,7 +250,7 @@ int plan(const uint16_t* a, int lda, const uint16_t* b, int ldb, long long b_row
   if (out->ws_bytes > mi::capi::kMaxWorkspace)
     return fail(MI_E_RANGE, "split-K workspace of %zu bytes exceeds %llu", out->ws_bytes, mi::capi::kMaxWorkspace);
   out->mm = EpiMM{a, b, (uint32_t)((size_t)M * lda * 2), (uint32_t)((size_t)b_rows * ldb * 2), M, N, K, lda, ldb,
-                  c.group_m > 0 ? c.group_m : 8, c.split_k, 0, 0, 0, 0};
+                  c.group_m > 0 ? c.group_m : 8, c.split_k};
   return MI_OK;
 }
 int run(const Product& p, const EpiOut& o, float* ws, hipStream_t s) {

@@ -3,32 +3,38 @@
 #pragma once
 #include "mi_mm_epi.hpp"
 
-// block_m, block_n, block_k, waves, lds_stages, rhs read non-temporally
-#define MI_EPI_CONFIGS(X)   \
-  X(256, 256, 64, 8, 2, 0)  \
-  X(256, 128, 64, 8, 3, 0)  \
-  X(256, 128, 64, 4, 2, 0)  \
-  X(256, 128, 64, 8, 2, 0)  \
-  X(128, 256, 64, 8, 3, 0)  \
-  X(128, 256, 64, 4, 2, 0)  \
-  X(128, 128, 64, 4, 2, 0)  \
-  X(128, 128, 64, 4, 4, 0)  \
-  X(64, 128, 64, 4, 2, 0)   \
-  X(64, 128, 64, 4, 3, 0)   \
-  X(128, 64, 64, 4, 2, 0)   \
-  X(128, 64, 64, 4, 3, 0)   \
-  X(64, 64, 64, 4, 2, 0)    \
-  X(64, 64, 64, 4, 4, 0)    \
-  X(32, 64, 64, 2, 4, 0)    \
-  X(32, 128, 64, 4, 4, 1)   \
-  X(64, 128, 64, 4, 4, 1)   \
-  X(128, 128, 64, 4, 2, 1)  \
-  X(128, 128, 64, 4, 3, 1)
+// block_m, block_n, block_k, waves, lds_stages, rhs read non-temporally;
+// then what the library's choice goes by, in microseconds: a K tile of a
+// block alone on its compute unit, a K tile of one of several that share it,
+// a block's beginning and end; and how many of its blocks a unit holds.
+//
+// Fitted (least squares of the logarithm, near the fastest config of each
+// shape) to these and eight more configs with up to 16 parts, timed at 44
+// shapes from 1 x 1024 x 1024 to 8192^3 in both layouts with bias and
+// gelu_tanh: the choice is within 1.014 of the fastest on average and 1.15 at
+// most (8 x 1024 x 4096, 1.1 us).  A large block alone is faster per flop but
+// leaves units idle in its last round, and a small one reads its operands
+// more often: 256x256 takes 102 us at 4096^3 where 128x128 takes 125; at
+// 1024^3 64x64 takes 6.9 us and 128x128 11.  Non-temporal reads of a weight
+// that is streamed once: 80.6 against 83.0 us at 16x28672x8192.
+#define MI_EPI_CONFIGS(X)                                 \
+  X(256, 256, 64, 8, 2, 0, 0.564f, 1.304f, 11.831f, 1)    \
+  X(256, 128, 64, 8, 3, 0, 0.720f, 0.413f, 6.953f, 1)     \
+  X(128, 256, 64, 8, 3, 0, 0.719f, 0.667f, 6.492f, 1)     \
+  X(128, 128, 64, 4, 4, 0, 0.457f, 0.294f, 5.173f, 1)     \
+  X(64, 128, 64, 4, 3, 0, 0.316f, 0.275f, 4.365f, 2)      \
+  X(128, 64, 64, 4, 3, 0, 0.318f, 0.264f, 4.439f, 2)      \
+  X(64, 64, 64, 4, 2, 0, 0.176f, 0.206f, 3.076f, 4)       \
+  X(64, 64, 64, 4, 4, 0, 0.144f, 0.186f, 3.255f, 2)       \
+  X(32, 128, 64, 4, 4, 1, 0.171f, 0.376f, 1.655f, 2)      \
+  X(128, 128, 64, 4, 3, 1, 0.575f, 0.350f, 4.790f, 1)
 
 namespace mi {
 
 struct EpiEntry {
   mi_tile_cfg cfg;  // split_k, group_m aside
+  float alone, shared, ends;
+  int per_cu;
   void (*direct)(const EpiMM&, const EpiOut&, hipStream_t);
   void (*split)(const EpiMM&, float* ws, int ldw, hipStream_t);
 };
@@ -51,6 +57,6 @@ void epi_split(const EpiMM& p, float* ws, int ldw, hipStream_t s) {
 
 }  // namespace mi
 
-#define MI_EPI_ROW(BM, BN, BK, W, S, NT)                                                   \
-  EpiEntry{mi_tile_cfg{BM, BN, BK, W, S, 1, 8, NT}, &epi_direct<BM, BN, BK, W, S, MI_EPI_BT, NT != 0>, \
-           &epi_split<BM, BN, BK, W, S, MI_EPI_BT, NT != 0>},
+#define MI_EPI_ROW(BM, BN, BK, W, S, NT, ALONE, SHARED, ENDS, PER_CU)                                           \
+  EpiEntry{mi_tile_cfg{BM, BN, BK, W, S, 1, 8, NT}, ALONE, SHARED, ENDS, PER_CU,                                \
+           &epi_direct<BM, BN, BK, W, S, MI_EPI_BT, NT != 0>, &epi_split<BM, BN, BK, W, S, MI_EPI_BT, NT != 0>},

@@ -18,10 +18,6 @@
 // and outputs is a 16-byte piece of a whole line, and the values are rounded
 // once, after the last operation.  Residual rows are requested before the
 // turn and arrive behind it.
-//
-// SEG3: A and B are each two bf16 planes, hi + lo (lo `plane` elements after
-// hi), and the K loop runs three times over: hi.hi, hi.lo, lo.hi.  lo.lo is
-// under 2^-18 of the product and left out.
 #pragma once
 #include <type_traits>
 
@@ -30,15 +26,12 @@
 
 namespace mi {
 
-// Operands as the kernel reads them.  K is a multiple of 8 (SEG3: of BK), lda
-// and ldb too; a_bytes, b_bytes: what lies behind the pointers (reads past it
+// Operands as the kernel reads them.  K, lda and ldb are multiples of 8; a_bytes, b_bytes: what lies behind the pointers (reads past it
 // give 0).
 struct EpiMM {
   const uint16_t *a, *b;
   uint32_t a_bytes, b_bytes;
   int M, N, K, lda, ldb, group_m, parts;
-  uint32_t plane_a, plane_b;          // SEG3: bytes from hi to lo
-  long long batch_a, batch_b;         // elements from one product's operand to the next's (blockIdx.y)
 };
 
 // TM x TN fragments of 16 rows and 16 columns a wave.
@@ -52,7 +45,7 @@ struct EpiCfg {
   // address then fits its 16 bits (with A and B of a stage together, the
   // second stage of a 256x256 block took a register per read).
   static constexpr int B_OFF = STAGES * A_BYTES;
-  static constexpr int TURN_COLS = TN >= 4 ? 64 : 32;
+  static constexpr int TURN_COLS = TN % 4 == 0 ? 64 : 32;
   static constexpr int TURN_ROW = TURN_COLS * 4 + 16;  // + 16: rows start in different banks
   static constexpr int TURN_BYTES = WAVES * 32 * TURN_ROW;
   static constexpr int MAIN_BYTES = STAGES * (A_BYTES + B_BYTES);
@@ -99,11 +92,12 @@ struct EpiKLoad {
                   tail ? voff_tail : voff);
   }
 };
-// 64 rows of COLS consecutive n (N contiguous).
-template <int COLS, int WAVES>
+// ROWS rows of COLS consecutive n (N contiguous).
+template <int COLS, int WAVES, int ROWS>
 struct EpiNLoad {
-  static constexpr int LOADS = COLS / 8 / WAVES, ROWB = COLS * 2, RPL = 1024 / ROWB;
-  static_assert(LOADS >= 1 && COLS % (8 * WAVES) == 0 && 2 * WAVES * RPL % 16 == 0, "whole loads, two swizzles");
+  static constexpr int LOADS = ROWS * COLS / 512 / WAVES, ROWB = COLS * 2, RPL = 1024 / ROWB;
+  static_assert(LOADS >= 1 && ROWS * COLS % (512 * WAVES) == 0 && RPL >= 1 && 2 * WAVES * RPL % 16 == 0,
+                "whole loads, two swizzles");
   uint32_t voff[2], first, step;
   int lds;
   __device__ __forceinline__ void init(int wave, int lane, int col0, int ld, int) {
@@ -124,7 +118,7 @@ struct EpiNLoad {
 // acc = the products of K tiles [kt0, kt0 + kts) of block (tm, tn).  Lane l,
 // register r of acc[i][j]: row 16 i + l % 16, column 16 j + 4 (l / 16) + r of
 // the wave's part.
-template <int BM, int BN, int BK, int WAVES, int STAGES, bool BT, bool NTB, bool SEG3, int TM, int TN>
+template <int BM, int BN, int BK, int WAVES, int STAGES, bool BT, bool NTB, int TM, int TN>
 __device__ __forceinline__ void epi_main(const EpiMM& p, const uint16_t* a, const uint16_t* b, char* smem, int tmi,
                                          int tni, int kt0, int kts, f32x4_t (&acc)[TM][TN]) {
   using C = EpiCfg<BM, BN, BK, WAVES, STAGES>;
@@ -134,7 +128,7 @@ __device__ __forceinline__ void epi_main(const EpiMM& p, const uint16_t* a, cons
   static_assert(C::LDS_BYTES <= kLdsBytesMax, "LDS over 160 KiB");
   constexpr int KS = BK / 32, NF = TM + TN, NM = TM * TN;
   using LA = EpiKLoad<BM, WAVES>;
-  using LB = std::conditional_t<BT, EpiKLoad<BN, WAVES>, EpiNLoad<BN, WAVES>>;
+  using LB = std::conditional_t<BT, EpiKLoad<BN, WAVES>, EpiNLoad<BN, WAVES, BK>>;
   constexpr int LPT = LA::LOADS + LB::LOADS;  // of every wave: vm_wait counts them
   static_assert((STAGES - 1) * LPT < 64, "loads in flight exceed the 6-bit vmcnt");
 
@@ -142,7 +136,7 @@ __device__ __forceinline__ void epi_main(const EpiMM& p, const uint16_t* a, cons
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m0 = tmi * BM, n0 = tni * BN;
   const int wm0 = (wave / G::WN) * G::WTM, wn0 = (wave % G::WN) * G::WTN;
-  const int KT1 = (p.K + BK - 1) / BK;  // K tiles of one pass over K
+  const int KT1 = (p.K + BK - 1) / BK;
   const int k_last = p.K - (KT1 - 1) * BK;
   LA la;
   LB lb;
@@ -207,19 +201,12 @@ __device__ __forceinline__ void epi_main(const EpiMM& p, const uint16_t* a, cons
   // Load q (< LPT) of K tile t of this block's range into `stage`.
   auto issue_one = [&](int q, int t, int stage) __attribute__((always_inline)) {
     const int kt = kt0 + t;
-    int r = kt, hi_a = 0, hi_b = 0;
-    if constexpr (SEG3) {
-      hi_a = kt >= 2 * KT1;
-      hi_b = kt >= KT1 && !hi_a;
-      r = kt - (hi_a ? 2 * KT1 : hi_b ? KT1 : 0);
-    }
-    const bool tail = !SEG3 && kt == KT1 - 1;
+    const bool tail = kt == KT1 - 1;
     if (q < LA::LOADS) {
-      const uint32_t off = (uint32_t)r * (uint32_t)(BK * 2) + (SEG3 && hi_a ? p.plane_a : 0u);
+      const uint32_t off = (uint32_t)kt * (uint32_t)(BK * 2);
       la.template issue<false>(q, a, p.a_bytes, off, smem + stage * C::A_BYTES, tail);
     } else {
-      const uint32_t off = (uint32_t)r * (BT ? (uint32_t)(BK * 2) : (uint32_t)BK * (uint32_t)p.ldb * 2u) +
-                           (SEG3 && hi_b ? p.plane_b : 0u);
+      const uint32_t off = (uint32_t)kt * (BT ? (uint32_t)(BK * 2) : (uint32_t)BK * (uint32_t)p.ldb * 2u);
       lb.template issue<NTB>(q - LA::LOADS, b, p.b_bytes, off, smem + C::B_OFF + stage * C::B_BYTES, tail);
     }
   };
@@ -329,10 +316,14 @@ __device__ __forceinline__ void epi_main(const EpiMM& p, const uint16_t* a, cons
 // the rows of turn s+1 are requested before the stores of turn s, and f has
 // no branch around a load or store, which would make the compiler wait for
 // all of them.
-template <int TM, int TN, int ROWB, class F>
+//
+// TURNED: f.apply_turned(n, m, v) also gets the values that apply left, 8 rows
+// m .. m + 7 (from the result's first row on, block_row the block's first) of
+// one column n.
+template <int TM, int TN, int ROWB, bool TURNED = false, class F>
 __device__ __forceinline__ void epi_rows(const f32x4_t (&acc)[TM][TN], char* smem, int wave, int lane, int row0,
-                                         int col0, F& f) {
-  constexpr int TW = TN >= 4 ? 2 : 1, LPR = 4 * TW, RPI = 64 / LPR, IT = 32 / RPI, NP = TN / (2 * TW), MT = TM / 2;
+                                         int col0, F& f, int block_row = 0) {
+  constexpr int TW = TN % 4 == 0 ? 2 : 1, LPR = 4 * TW, RPI = 64 / LPR, IT = 32 / RPI, NP = TN / (2 * TW), MT = TM / 2;
   static_assert(TN % (2 * TW) == 0 && TM % 2 == 0 && ROWB == TW * 128 + 16 && IT <= 4, "turn layout");
   MI_LDS char* slot = (MI_LDS char*)smem + wave * (32 * ROWB);
   const int n0 = col0 + 8 * (lane % LPR), r0 = row0 + lane / LPR;
@@ -366,8 +357,26 @@ __device__ __forceinline__ void epi_rows(const f32x4_t (&acc)[TM][TN], char* sme
         const f32x4_t lo = *(MI_LDS f32x4_t*)at, hi = *(MI_LDS f32x4_t*)(at + 16);
         float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
         f.apply(it, r0 + mt * 32 + it * RPI, n, v);
+        if constexpr (TURNED) {
+          *(MI_LDS f32x4_t*)at = f32x4_t{v[0], v[1], v[2], v[3]};
+          *(MI_LDS f32x4_t*)(at + 16) = f32x4_t{v[4], v[5], v[6], v[7]};
+        }
       }
       wave_lds_turn();
+      if constexpr (TURNED) {
+        // A lane per column: neighbours read neighbouring words of a row.
+        constexpr int W = TW * 32, LANES = 64 / W;
+        const int c = lane % W;
+#pragma unroll
+        for (int g = 0; g < 4 / LANES; ++g) {
+          const int r = 8 * (g * LANES + lane / W);
+          float v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = *(MI_LDS float*)(slot + (r + i) * ROWB + 4 * c);
+          f.apply_turned(col0 + np * W + c, block_row + row0 + mt * 32 + r, v);
+        }
+        wave_lds_turn();
+      }
     }
   }
 }
@@ -539,7 +548,7 @@ __global__ __launch_bounds__(WAVES * 64) void mm_epi_kernel(const EpiMM p, EpiOu
   int tm, tn;
   tile_coords((p.M + BM - 1) / BM, (p.N + BN - 1) / BN, p.group_m, tm, tn);
   f32x4_t acc[C::TM][C::TN];
-  epi_main<BM, BN, BK, WAVES, STAGES, BT, NTB, false>(p, p.a, p.b, smem, tm, tn, 0, (p.K + BK - 1) / BK, acc);
+  epi_main<BM, BN, BK, WAVES, STAGES, BT, NTB>(p, p.a, p.b, smem, tm, tn, 0, (p.K + BK - 1) / BK, acc);
   const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int row0 = (wave / G::WN) * G::WTM, col0 = tn * BN + (wave % G::WN) * G::WTN;
   if (e.vec) {
@@ -582,7 +591,7 @@ __global__ __launch_bounds__(WAVES * 64) void mm_epi_split_kernel(const EpiMM p,
   tile_coords_split((p.M + BM - 1) / BM, (p.N + BN - 1) / BN, p.group_m, p.parts, tm, tn, part);
   const int KT = (p.K + BK - 1) / BK, each = (KT + p.parts - 1) / p.parts, kt0 = part * each;
   f32x4_t acc[C::TM][C::TN];
-  epi_main<BM, BN, BK, WAVES, STAGES, BT, NTB, false>(p, p.a, p.b, smem, tm, tn, kt0, KT - kt0 < each ? KT - kt0 : each,
+  epi_main<BM, BN, BK, WAVES, STAGES, BT, NTB>(p, p.a, p.b, smem, tm, tn, kt0, KT - kt0 < each ? KT - kt0 : each,
                                                       acc);
   const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   EpiPart f;

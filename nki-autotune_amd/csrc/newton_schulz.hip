@@ -7,7 +7,7 @@
 namespace {
 
 using mi::Bf16;
-using mi::EpiMM;
+using mi::NsMM;
 using mi::NsOut;
 using mi::capi::fail;
 
@@ -36,8 +36,9 @@ __global__ __launch_bounds__(256) void ns_square_kernel(const T* __restrict__ g,
   if (threadIdx.x == 0) part[(size_t)blockIdx.y * gridDim.x + blockIdx.x] = ((xs[0] + xs[1]) + xs[2]) + xs[3];
 }
 
-// The planes of X_0 = G / (||G|| + eps), or of G^T: 64 x 64 pieces, turned in
-// LDS.  G [m][n]; X [s][2 * lp], s x l of it G's or G^T's, the rest zeros.
+// X_0 = G / (||G|| + eps), or of G^T: 64 x 64 pieces, turned in LDS.  G
+// [m][n]; X [s][2 * lp] (hi and lo by 32), s x l of it G's or G^T's, the rest
+// zeros.
 struct NsInit {
   const void* g;
   uint16_t* x;
@@ -49,10 +50,18 @@ struct NsInit {
 template <class T>
 __global__ __launch_bounds__(256) void ns_init_kernel(const NsInit p) {
   __shared__ float tile[64][65];
-  __shared__ double sums[kNormBlocks];
   __shared__ float scale_lds;
   const int tid = (int)threadIdx.x, z = (int)blockIdx.z;
-  if (tid < p.parts) sums[tid] = p.part[(size_t)z * p.parts + tid];
+  if (tid < 64) {
+    // The parts' sum, in an order fixed by their number.
+    double t[kNormBlocks / 64];
+#pragma unroll
+    for (int i = 0; i < kNormBlocks / 64; ++i)
+      t[i] = tid + 64 * i < p.parts ? p.part[(size_t)z * p.parts + tid + 64 * i] : 0.0;
+    double sum = (t[0] + t[1]) + (t[2] + t[3]);
+    for (int k = 32; k > 0; k >>= 1) sum += __shfl_xor(sum, k);
+    if (tid == 0) scale_lds = (float)(1.0 / (__builtin_sqrt(sum) + (double)p.eps));
+  }
   const T* g = (const T*)p.g + (size_t)z * (size_t)p.m * (size_t)p.n;
   const int r0 = (int)blockIdx.y * 64, c0 = (int)blockIdx.x * 64;  // of X
   for (int i = tid; i < 64 * 64; i += 256) {
@@ -63,17 +72,11 @@ __global__ __launch_bounds__(256) void ns_init_kernel(const NsInit p) {
     else tile[a][b] = v;
   }
   __syncthreads();
-  if (tid == 0) {
-    double t = 0.0;
-    for (int i = 0; i < p.parts; ++i) t += sums[i];
-    scale_lds = (float)(1.0 / (__builtin_sqrt(t) + (double)p.eps));
-  }
-  __syncthreads();
   const float scale = scale_lds;
   uint16_t* x = p.x + (size_t)z * (size_t)p.s * (size_t)(2 * p.lp);
   for (int i = tid; i < 64 * 8; i += 256) {
     const int r = i / 8, c = (i % 8) * 8;
-    if (r0 + r >= p.s) continue;
+    if (r0 + r >= p.s || c0 + c >= p.lp) continue;
     float v[8], t[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = tile[r][c + k] * scale;
@@ -81,14 +84,14 @@ __global__ __launch_bounds__(256) void ns_init_kernel(const NsInit p) {
     mi::unpack8(hi, t);
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] -= t[k];
-    uint16_t* at = x + (size_t)(r0 + r) * (size_t)(2 * p.lp) + c0 + c;
+    uint16_t* at = x + (size_t)(r0 + r) * (size_t)(2 * p.lp) + mi::ns_at(c0 + c);
     *(mi::u32x4_t*)at = hi;
-    *(mi::u32x4_t*)(at + p.lp) = mi::pack8(v);
+    *(mi::u32x4_t*)(at + 32) = mi::pack8(v);
   }
 }
 
-// out [m][n] from the hi plane of X [s][2 * lp], turned back where G was.
-// hi is the value rounded to bf16.
+// out [m][n] from the hi values of X [s][2 * lp], turned back where G was: hi
+// is the value rounded to bf16.
 __global__ __launch_bounds__(256) void ns_last_kernel(const uint16_t* __restrict__ x, uint16_t* __restrict__ out, int m,
                                                       int n, int s, int lp, bool turn) {
   __shared__ uint16_t tile[64][66];
@@ -99,7 +102,7 @@ __global__ __launch_bounds__(256) void ns_last_kernel(const uint16_t* __restrict
     const int a = i / 64, b = i % 64;
     const int row = (turn ? c0 : r0) + a, col = (turn ? r0 : c0) + b;  // of X
     const bool in = row < s && col < lp;
-    const uint16_t v = in ? src[(size_t)row * (size_t)(2 * lp) + col] : (uint16_t)0;
+    const uint16_t v = in ? src[(size_t)row * (size_t)(2 * lp) + mi::ns_at(col)] : (uint16_t)0;
     if (turn) tile[b][a] = v;
     else tile[a][b] = v;
   }
@@ -135,12 +138,12 @@ int ns_plan(const mi_newton_schulz_args* p, Plan* q) {
   q->s = q->turn ? p->n : p->m;
   q->l = q->turn ? p->m : p->n;
   // A matrix's planes, and a block of rows past them, within 32-bit offsets.
-  const unsigned long long lp = ((unsigned long long)q->l + 63) / 64 * 64;
+  const unsigned long long lp = ((unsigned long long)q->l + 31) / 32 * 32;
   if (((unsigned long long)q->s + 512) * lp * 4 > mi::capi::kMaxOffset)
     return fail(MI_E_RANGE, "the planes of a %d x %d matrix exceed 32-bit buffer offsets", p->m, p->n);
-  if (lp / 64 > 65535) return fail(MI_E_RANGE, "a side of %d exceeds 64 * 65535", q->l);
+  if (q->l > 1 << 20) return fail(MI_E_RANGE, "a side of %d exceeds %d", q->l, 1 << 20);
   q->lp = (int)lp;
-  q->sp = (q->s + 63) / 64 * 64;
+  q->sp = (q->s + 31) / 32 * 32;
   const long long n = (long long)p->m * p->n;
   q->parts = (int)(n / 2048 < 1 ? 1 : n / 2048 > kNormBlocks ? kNormBlocks : n / 2048);
   const size_t x = up256((size_t)p->batch * q->s * q->lp * 4), a = up256((size_t)p->batch * q->s * q->sp * 4);
@@ -152,18 +155,61 @@ int ns_plan(const mi_newton_schulz_args* p, Plan* q) {
   return MI_OK;
 }
 
-template <int BM, int BN, int BK, int W, int S, bool BT>
-int product(const EpiMM& p, const NsOut& o, int batch, hipStream_t s) {
-  const unsigned tiles = (unsigned)((p.M + BM - 1) / BM) * (unsigned)((p.N + BN - 1) / BN);
-  mi::ns_product_kernel<BM, BN, BK, W, S, BT><<<dim3(tiles, (unsigned)batch), dim3(W * 64), 0, s>>>(p, o);
+template <int BM, int BN, int W, int S, bool BT, bool SYM>
+int product(const NsMM& p, const NsOut& o, int batch, hipStream_t s) {
+  const unsigned tm = (unsigned)((p.M + BM - 1) / BM), tn = (unsigned)((p.N + BN - 1) / BN);
+  mi::ns_product_kernel<BM, BN, W, S, BT, SYM>
+      <<<dim3(SYM ? tn * (tn + 1) / 2 : tm * tn, (unsigned)batch), dim3(W * 64), 0, s>>>(p, o);
   return launched("Newton-Schulz product");
 }
-template <bool BT>
-int product(const EpiMM& p, const NsOut& o, int batch, hipStream_t s) {
-  const auto tiles = [&](int b) { return (long long)batch * ((p.M + b - 1) / b) * ((p.N + b - 1) / b); };
-  if (tiles(256) >= 200) return product<256, 256, 64, 8, 2, BT>(p, o, batch, s);
-  if (tiles(128) >= 200) return product<128, 128, 64, 4, 4, BT>(p, o, batch, s);
-  return product<64, 64, 64, 4, 4, BT>(p, o, batch, s);
+// Which block a product takes: the least estimated time, a K tile of a block
+// alone on its unit (`alone`) or of one of several (`shared`), and a block's
+// ends, in microseconds, fitted to five steps timed at 15 sizes from 128 x 128
+// to 4096 x 4096 and 32 of 512 x 512.  Small blocks fill the chip where there
+// are few (1024 x 1024: 182 us with 64-wide blocks, 301 with 128), large ones
+// read their operands less often (4096 x 4096: 5.55 ms with 64, 4.05 with 192
+// and 256).  The choice was within 1.06 of the fastest of each size.
+struct NsBlock {
+  int bm, per_cu;
+  double alone, shared, ends;
+};
+double estimate(const NsBlock& b, long long blocks, int kts, int cus) {
+  const long long each = (blocks + cus - 1) / cus, rounds = (each + b.per_cu - 1) / b.per_cu;
+  const double in_line = (double)each * b.shared * kts, alone = (double)rounds * b.alone * kts;
+  return (in_line > alone ? in_line : alone) + (double)rounds * b.ends;
+}
+template <size_t N>
+int fastest(const NsBlock (&b)[N], const NsMM& p, bool sym, int batch) {
+  const int cus = mi::capi::device_cus();
+  int best = 0;
+  double least = 1e30;
+  for (size_t i = 0; i < N; ++i) {
+    const long long tm = (p.M + b[i].bm - 1) / b[i].bm, tn = (p.N + b[i].bm - 1) / b[i].bm;
+    const double us = estimate(b[i], batch * (sym ? tn * (tn + 1) / 2 : tm * tn), p.kw / 32, cus);
+    if (us < least) {
+      least = us;
+      best = b[i].bm;
+    }
+  }
+  return best;
+}
+int symmetric(const NsMM& p, const NsOut& o, int batch, hipStream_t s) {
+  static constexpr NsBlock blocks[] = {
+      {64, 2, 0.205, 0.235, 3.875}, {128, 1, 0.538, 0.467, 6.619}, {192, 1, 0.949, 1.036, 12.722}};
+  switch (fastest(blocks, p, true, batch)) {
+    case 64: return product<64, 64, 4, 4, true, true>(p, o, batch, s);
+    case 128: return product<128, 128, 4, 4, true, true>(p, o, batch, s);
+    default: return product<192, 192, 4, 3, true, true>(p, o, batch, s);
+  }
+}
+int update(const NsMM& p, const NsOut& o, int batch, hipStream_t s) {
+  static constexpr NsBlock blocks[] = {
+      {64, 2, 0.219, 0.178, 6.251}, {128, 2, 0.543, 0.597, 6.950}, {256, 1, 1.478, 1.533, 11.596}};
+  switch (fastest(blocks, p, false, batch)) {
+    case 64: return product<64, 64, 4, 4, false, false>(p, o, batch, s);
+    case 128: return product<128, 128, 4, 2, false, false>(p, o, batch, s);
+    default: return product<256, 256, 8, 2, false, false>(p, o, batch, s);
+  }
 }
 
 }  // namespace
@@ -202,7 +248,7 @@ int mi_newton_schulz(const mi_newton_schulz_args* args, void* workspace, unsigne
   const long long per = (long long)m * n;
   const dim3 sq((unsigned)q.parts, (unsigned)batch);
   const NsInit init = {args->grad, x, part, q.parts, m, n, q.s, q.l, q.lp, args->eps, q.turn};
-  const dim3 ig((unsigned)(q.lp / 64), (unsigned)((q.s + 63) / 64), (unsigned)batch);
+  const dim3 ig((unsigned)((q.lp + 63) / 64), (unsigned)((q.s + 63) / 64), (unsigned)batch);
   if (args->dtype == MI_DTYPE_F32) {
     ns_square_kernel<float><<<sq, dim3(256), 0, st>>>((const float*)args->grad, part, per);
     if ((rc = launched("sum of squares")) != MI_OK) return rc;
@@ -218,16 +264,16 @@ int mi_newton_schulz(const mi_newton_schulz_args* args, void* workspace, unsigne
   const long long xz = (long long)s * lp * 2, az = (long long)s * sp * 2;
   const bool direct = !q.turn && n == lp && (uintptr_t)args->out % 16 == 0;  // the last product stores out itself
   for (int k = 0; k < args->steps; ++k) {
-    const EpiMM gram = {x, x, xb, xb, s, sp, lp, 2 * lp, 2 * lp, 8, 1, (uint32_t)lp * 2, (uint32_t)lp * 2, xz, xz};
-    const NsOut to_a = {nullptr, A, nullptr, s, sp, 2 * sp, 1.0f, 0.0f, 0, az, 0};
-    if ((rc = product<true>(gram, to_a, batch, st)) != MI_OK) return rc;
-    const EpiMM square = {A, A, ab, ab, s, sp, sp, 2 * sp, 2 * sp, 8, 1, (uint32_t)sp * 2, (uint32_t)sp * 2, az, az};
-    const NsOut to_b = {A, B, nullptr, s, sp, 2 * sp, args->c, args->b, az, az, 0};
-    if ((rc = product<true>(square, to_b, batch, st)) != MI_OK) return rc;
-    const EpiMM update = {B, x, ab, xb, s, lp, sp, 2 * sp, 2 * lp, 8, 1, (uint32_t)sp * 2, (uint32_t)lp * 2, az, xz};
+    const NsMM gram = {x, x, xb, xb, s, sp, lp, lp, lp, xz, xz};
+    const NsOut to_a = {nullptr, A, nullptr, s, sp, 1.0f, 0.0f, 0, az, 0};
+    if ((rc = symmetric(gram, to_a, batch, st)) != MI_OK) return rc;
+    const NsMM square = {A, A, ab, ab, s, sp, sp, sp, sp, az, az};
+    const NsOut to_b = {A, B, nullptr, s, sp, args->c, args->b, az, az, 0};
+    if ((rc = symmetric(square, to_b, batch, st)) != MI_OK) return rc;
+    const NsMM by_b = {B, x, ab, xb, s, lp, sp, sp, lp, az, xz};
     const bool last = direct && k + 1 == args->steps;
-    const NsOut to_x = {x, last ? nullptr : next, last ? (uint16_t*)args->out : nullptr, s, lp, 2 * lp, 1.0f, args->a, xz, xz, per};
-    if ((rc = product<false>(update, to_x, batch, st)) != MI_OK) return rc;
+    const NsOut to_x = {x, last ? nullptr : next, last ? (uint16_t*)args->out : nullptr, s, lp, 1.0f, args->a, xz, xz, per};
+    if ((rc = update(by_b, to_x, batch, st)) != MI_OK) return rc;
     uint16_t* t = x;
     x = next;
     next = t;
