@@ -89,11 +89,11 @@ def _link(objs: list[Path], lib: Path) -> None:
 
 
 def _build_torch_call(force: bool) -> None:
-    """csrc/host/mi_torch_call.cpp -> kernel_library/_torch_call.so (g++ against the installed torch).
+    """csrc/host/*.cpp -> kernel_library/_torch_call.so (g++ against the installed torch).
 
     Built again when a source is newer, or when it was built for another torch or Python than the running ones."""
-    src = CSRC / "host" / "mi_torch_call.cpp"
-    deps = [src, *INCLUDE.glob("*.h")]
+    srcs = sorted((CSRC / "host").glob("*.cpp"))
+    deps = [*srcs, *(CSRC / "host").glob("*.hpp"), *INCLUDE.glob("*.h")]
     stamp = BUILD / "torch_call.for"
     built_for = f"torch {metadata.version('torch')}, Python {sys.version.split()[0]}"
     if (not force and TORCH_CALL.exists() and stamp.exists() and stamp.read_text() == built_for
@@ -107,11 +107,11 @@ def _build_torch_call(force: bool) -> None:
              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
     paths = [*cpp_extension.include_paths("cuda"), sysconfig.get_paths()["include"]]
     tmp = TORCH_CALL.with_suffix(".so.tmp")
-    cmd = ["g++", *flags, *(f"-I{p}" for p in paths), str(src), "-o", str(tmp),
+    cmd = ["g++", *flags, *(f"-I{p}" for p in paths), *map(str, srcs), "-o", str(tmp),
            f"-L{Path(torch.__file__).parent / 'lib'}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
-        raise RuntimeError(f"g++ failed for {src.name}:\n{proc.stdout}{proc.stderr}")
+        raise RuntimeError(f"g++ failed for {TORCH_CALL.name}:\n{proc.stdout}{proc.stderr}")
     os.replace(tmp, TORCH_CALL)
     stamp.write_text(built_for)
 

@@ -17,15 +17,6 @@
 // Nothing is kept between calls but the shapes' configs: no pointer, tensor
 // or identity.  The GIL is held throughout except around the launch, as
 // ctypes does, so the table needs no lock; nothing shared is read there.
-#include <ATen/ATen.h>
-#include <ATen/PythonTorchFunctionTLS.h>
-#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
-#include <Python.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/core/impl/LocalDispatchKeySet.h>
-#include <c10/core/impl/TorchDispatchModeTLS.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/python_variable.h>
 #include <torch/version.h>
 
 #include <climits>
@@ -36,8 +27,15 @@
 #include <unordered_map>
 
 #include "../../../include/mi_kernels.h"
+#include "mi_torch_plain.hpp"
+
+extern PyMethodDef kOperatorMethods[];  // mi_operator_call.cpp
 
 namespace {
+
+using mi_torch::disjoint;
+using mi_torch::no_mode;
+using mi_torch::plain;
 
 // What a call computes; the first argument of call() and remember().
 enum Kind { kLhsTBf16 = 0, kLhsTF32 = 1, kRms = 2, kLhs = 3, kRmsNoGamma = 4 };
@@ -65,33 +63,6 @@ struct ShapeHash {
 };
 constexpr size_t kMaxShapes = 1 << 16;
 std::unordered_map<Shape, mi_tile_cfg, ShapeHash> g_configs;
-
-// A dense tensor on a HIP device that nothing intercepts: an exact Tensor or
-// Parameter whose dispatch keys are the device's own, autograd's and
-// autocast's (no conjugate or negative view, no functorch, Python or sparse
-// key).
-const at::Tensor* plain(PyObject* o, at::ScalarType dtype) {
-  if (!THPVariable_CheckExact(o)) return nullptr;
-  const at::Tensor& t = THPVariable_Unpack(o);
-  static const uint64_t allowed =
-      (c10::DispatchKeySet(c10::DispatchKey::CUDA) | c10::DispatchKeySet(c10::DispatchKey::AutogradCUDA) |
-       c10::DispatchKeySet(c10::DispatchKey::ADInplaceOrView) | c10::autocast_dispatch_keyset).raw_repr();
-  if (!t.defined() || (t.key_set().raw_repr() & ~allowed) != 0) return nullptr;
-  if (!t.is_cuda() || t.scalar_type() != dtype || !t.is_contiguous()) return nullptr;
-  return &t;
-}
-
-// No mode or transform is active on this thread.
-bool no_mode() {
-  if (at::impl::torch_function_mode_enabled() || c10::impl::dispatch_mode_enabled()) return false;
-  static const uint64_t allowed = (c10::default_included_set | c10::autocast_dispatch_keyset).raw_repr();
-  return (c10::impl::tls_local_dispatch_key_set().included_.raw_repr() & ~allowed) == 0;
-}
-
-bool disjoint(const at::Tensor& out, const at::Tensor& in) {
-  const uintptr_t o = (uintptr_t)out.data_ptr(), i = (uintptr_t)in.data_ptr();
-  return o + out.nbytes() <= i || i + in.nbytes() <= o;
-}
 
 // call(kind, a, b, gamma | None, eps, out | None): the output tensor, or
 // None when the Python body has to run.  kind: 0 (bf16 or fp32 lhsT.rhs),
@@ -268,5 +239,8 @@ PyMODINIT_FUNC PyInit__torch_call() {
   const bool same = now && std::strncmp(now, TORCH_VERSION, n) == 0 && (now[n] == '\0' || now[n] == '+');
   if (now && !same) PyErr_Format(PyExc_ImportError, "built for torch %s, found %s", TORCH_VERSION, now);
   Py_DECREF(version);
-  return same ? PyModule_Create(&kModule) : nullptr;
+  if (!same) return nullptr;
+  PyObject* m = PyModule_Create(&kModule);
+  if (m && PyModule_AddFunctions(m, kOperatorMethods) < 0) Py_CLEAR(m);
+  return m;
 }

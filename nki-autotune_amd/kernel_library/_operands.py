@@ -3,11 +3,17 @@
 from __future__ import annotations
 
 import ctypes
+import os
 from collections.abc import Callable, Container
 
 import torch
 
 from kernel_library import _lib
+from kernel_library.config import _torch_call
+
+_ENTRY_POINTS = ("mi_layer_norm", "mi_layer_norm_backward_workspace", "mi_layer_norm_backward",
+                 "mi_matmul_epilogue_workspace", "mi_matmul_epilogue_bf16", "mi_matmul_epilogue_backward_workspace",
+                 "mi_matmul_epilogue_backward_bf16", "mi_newton_schulz_workspace", "mi_newton_schulz")
 
 
 def tensor(name: str, t: object, dtypes: Container[torch.dtype], ref: torch.Tensor | None = None,
@@ -53,7 +59,7 @@ def workspace(device: torch.device, what: str, query: Callable, *args) -> tuple[
 
 
 def launch(device: torch.device, what: str, fn: Callable, *args) -> None:
-    """``fn(*args, stream)`` on the current stream of ``device``."""
+    """``fn(*args, stream)`` on the current stream of ``device``; the native calls learn of the library that ran it."""
     stream = torch.cuda.current_stream(device).cuda_stream
     if device.index == torch.cuda.current_device():
         rc = fn(*args, stream)
@@ -61,3 +67,8 @@ def launch(device: torch.device, what: str, fn: Callable, *args) -> None:
         with torch.cuda.device(device):
             rc = fn(*args, stream)
     _lib.check_rc(rc, what)
+    if not _torch_call.knows_operators():
+        L = _lib.lib()
+        _torch_call.bind_operators(os.environ.get("MI_KERNELS_LIB", ""),
+                                   *(ctypes.cast(getattr(L, f), ctypes.c_void_p).value for f in _ENTRY_POINTS),
+                                   _lib.check_rc)

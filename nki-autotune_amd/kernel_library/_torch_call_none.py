@@ -26,3 +26,18 @@ def knows(kind, M, N, K):
 
 def forget():
     return None
+
+
+def layer_norm(*args):
+    return None
+
+
+layer_norm_backward = matmul_epilogue = matmul_epilogue_backward = newton_schulz = layer_norm
+
+
+def bind_operators(*entry_points):
+    return None
+
+
+def knows_operators():
+    return True  # nothing to bind

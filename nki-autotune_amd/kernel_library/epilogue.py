@@ -20,7 +20,7 @@ import torch
 
 from kernel_library import _lib
 from kernel_library._operands import launch, no_overlap, tensor, workspace
-from kernel_library.config import TileConfig
+from kernel_library.config import TileConfig, _torch_call
 
 _ACTIVATIONS = {None: _lib.MI_ACT_NONE, "none": _lib.MI_ACT_NONE, "relu": _lib.MI_ACT_RELU, "gelu": _lib.MI_ACT_GELU,
                 "gelu_tanh": _lib.MI_ACT_GELU_TANH, "silu": _lib.MI_ACT_SILU}
@@ -93,8 +93,12 @@ def matmul_epilogue(
     ``activation``: None, "relu", "gelu" (erf), "gelu_tanh" or "silu".  ``pre``, where given, gets ``lhs @ rhs + bias``,
     which the gradient of an activation takes.  ``cfg``: one of ``epilogue_configs()``, any ``split_k`` and
     ``group_m``; None for the library's choice."""
-    M, N, K = _operands(lhs, rhs, rhs_transposed)
     act = _activation(activation)
+    if cfg is None:
+        done = _torch_call.matmul_epilogue(lhs, rhs, bias, act, residual, rhs_transposed, pre, out)
+        if done is not None:
+            return done
+    M, N, K = _operands(lhs, rhs, rhs_transposed)
     f32 = _check_bias(bias, N, lhs)
     if residual is not None:
         _matrix("residual", residual, M, N, lhs)
@@ -131,8 +135,11 @@ def matmul_epilogue_backward(
     ``pre`` is what the forward call wrote, needed for an activation.  ``dbias`` has the bias's type and is None where
     it is (``bias`` is not read); the residual's gradient is ``dout`` itself.  Without ``need_dlhs`` or ``need_drhs``
     that gradient is None and not computed."""
-    M, N, K = _operands(lhs, rhs, rhs_transposed)
     act = _activation(activation)
+    done = _torch_call.matmul_epilogue_backward(dout, lhs, rhs, act, pre, bias, rhs_transposed, need_dlhs, need_drhs)
+    if done is not None:
+        return done
+    M, N, K = _operands(lhs, rhs, rhs_transposed)
     _matrix("dout", dout, M, N, lhs)
     if act != _lib.MI_ACT_NONE:
         if pre is None:

@@ -18,6 +18,7 @@ import torch
 
 from kernel_library import _lib
 from kernel_library._operands import launch, no_overlap, tensor, workspace
+from kernel_library.config import _torch_call
 
 _DTYPES = {torch.bfloat16: _lib.MI_DTYPE_BF16, torch.float16: _lib.MI_DTYPE_F16, torch.float32: _lib.MI_DTYPE_F32}
 
@@ -68,6 +69,9 @@ def layer_norm(
 
     With ``stats`` the call returns ``(y, mean, rstd)``, the rows' fp32 statistics that ``layer_norm_backward`` takes
     (of x's shape without its last dimension)."""
+    done = _torch_call.layer_norm(x, weight, bias, eps, out, stats)
+    if done is not None:
+        return done
     tensor("x", x, _DTYPES)
     rows, D, ldx = _rows("x", x)
     f32 = _params(x, D, weight, bias)
@@ -104,6 +108,9 @@ def layer_norm_backward(
 
     ``mean`` and ``rstd`` are what the forward call returned with ``stats``.  ``dweight`` and ``dbias`` have their
     parameter's type and are None where it is (``bias`` is not read); ``dx`` is None without ``need_dx``."""
+    done = _torch_call.layer_norm_backward(dout, x, mean, rstd, weight, bias, need_dx)
+    if done is not None:
+        return done
     tensor("x", x, _DTYPES)
     rows, D, ldx = _rows("x", x)
     tensor("dout", dout, {x.dtype}, x, "x")

@@ -15,6 +15,7 @@ import torch
 
 from kernel_library import _lib
 from kernel_library._operands import launch, no_overlap, tensor, workspace
+from kernel_library.config import _torch_call
 
 _DTYPES = {torch.bfloat16: _lib.MI_DTYPE_BF16, torch.float32: _lib.MI_DTYPE_F32}
 
@@ -30,11 +31,14 @@ def newton_schulz(
 
     ``grad``: ``[m, n]``, or ``[batch, m, n]`` for that many matrices, each by itself; bf16 or fp32, contiguous.
     ``coefficients``: ``(a, b, c)``."""
+    if len(coefficients) != 3:
+        raise ValueError(f"coefficients must be (a, b, c), got {coefficients!r}")
+    done = _torch_call.newton_schulz(grad, steps, *coefficients, eps, out)
+    if done is not None:
+        return done
     tensor("grad", grad, _DTYPES)
     if grad.dim() not in (2, 3) or not grad.is_contiguous():
         raise ValueError(f"grad must be contiguous, [m, n] or [batch, m, n], got shape {tuple(grad.shape)}")
-    if len(coefficients) != 3:
-        raise ValueError(f"coefficients must be (a, b, c), got {coefficients!r}")
     if steps < 0:
         raise ValueError(f"steps must be >= 0, got {steps}")
     if not 0.0 <= eps < 3e38:

@@ -1,0 +1,115 @@
+"""The native calls of the operators (csrc/host/mi_operator_call.cpp): they take ordinary calls, answer as the Python
+bodies do, and leave everything else to them."""
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+class _Python:
+    """The extension with its operators left to the Python bodies."""
+
+    def __init__(self, native):
+        self.native = native
+
+    def __getattr__(self, name):
+        if name in ("layer_norm", "layer_norm_backward", "matmul_epilogue", "matmul_epilogue_backward", "newton_schulz"):
+            return lambda *args: None
+        return getattr(self.native, name)
+
+
+def _both(monkeypatch, call):
+    """``call()`` by the native functions and by the Python bodies."""
+    from kernel_library import _operands, epilogue, norm, orthogonal
+
+    call()  # binds
+    native = _operands._torch_call
+    assert native.knows_operators()
+    fast = call()
+    with monkeypatch.context() as m:
+        for mod in (epilogue, norm, orthogonal):
+            m.setattr(mod, "_torch_call", _Python(native))
+        slow = call()
+    return fast, slow
+
+
+def _same(a, b):
+    if isinstance(a, (tuple, list)):
+        return type(a) is type(b) and len(a) == len(b) and all(_same(x, y) for x, y in zip(a, b))
+    if a is None or b is None:
+        return a is b
+    return a.dtype == b.dtype and a.shape == b.shape and not a.requires_grad and bool((a == b).all())
+
+
+def test_answers_are_the_python_bodies(gpu, monkeypatch):
+    import torch
+
+    import kernel_library as kl
+
+    bf = torch.bfloat16
+    x, w, b = (torch.randn(s, device=gpu).to(bf) for s in ((3, 5, 320), (320,), (320,)))
+    lhs, rhs = torch.randn(70, 96, device=gpu).to(bf), torch.randn(96, 136, device=gpu).to(bf)
+    bias, res, pre = torch.randn(136, device=gpu), torch.randn(70, 136, device=gpu).to(bf), torch.zeros(70, 136, device=gpu).to(bf)
+    param = torch.nn.Parameter(rhs)
+    y, mean, rstd = kl.layer_norm(x, w, b, stats=True)
+    calls = [
+        lambda: kl.layer_norm(x),
+        lambda: kl.layer_norm(x, w, b, 1e-3),
+        lambda: kl.layer_norm(x, w.float(), stats=True),
+        lambda: kl.layer_norm(x, w, b, out=torch.zeros_like(x)),
+        lambda: kl.layer_norm_backward(y, x, mean, rstd, w, b),
+        lambda: kl.layer_norm_backward(y, x, mean, rstd, None, b, need_dx=False),
+        lambda: kl.matmul_epilogue(lhs, param),
+        lambda: kl.matmul_epilogue(lhs, rhs, bias, "gelu", res, pre=pre),
+        lambda: kl.matmul_epilogue(lhs, rhs.t().contiguous(), bias.to(bf), "silu", rhs_transposed=True, out=torch.zeros_like(res)),
+        lambda: kl.matmul_epilogue_backward(res, lhs, param, "gelu", pre, bias),
+        lambda: kl.matmul_epilogue_backward(res, lhs, rhs, need_dlhs=False),
+        lambda: kl.newton_schulz(lhs),
+        lambda: kl.newton_schulz(x.float(), steps=2, coefficients=(1.5, -0.5, 0.0), eps=0.0, out=torch.zeros_like(x)),
+    ]
+    for i, call in enumerate(calls):
+        fast, slow = _both(monkeypatch, call)
+        assert _same(fast, slow), i
+
+
+def test_ordinary_calls_are_taken(gpu):
+    import torch
+
+    import kernel_library as kl
+    from kernel_library import _operands
+
+    t = torch.randn(16, 64, device=gpu).bfloat16()
+    kl.layer_norm(t[:, :8])  # the Python body binds
+    n = _operands._torch_call
+    assert n.layer_norm(t, None, None, 1e-5, None, False) is not None
+    assert n.matmul_epilogue(t, t, None, 0, None, True, None, None) is not None
+    assert n.newton_schulz(t, 5, 3.4445, -4.775, 2.0315, 1e-7, None) is not None
+    # Left to the Python body: another layout, type, device, an overlap, nothing to do.
+    assert n.layer_norm(t[:, :8], None, None, 1e-5, None, False) is None
+    assert n.layer_norm(t.double(), None, None, 1e-5, None, False) is None
+    assert n.layer_norm(t.cpu(), None, None, 1e-5, None, False) is None
+    assert n.layer_norm(t, None, None, 1e-5, t, False) is None
+    assert n.layer_norm(t, None, None, -1.0, None, False) is None
+    assert n.layer_norm(t, t[0, :8], None, 1e-5, None, False) is None
+    assert n.layer_norm(t[:0], None, None, 1e-5, None, False) is None
+    assert n.matmul_epilogue(t, t, None, 0, None, False, None, None) is None
+    assert n.matmul_epilogue(t, t, None, 0, None, True, None, t) is None
+    assert n.matmul_epilogue(t, t.float(), None, 0, None, True, None, None) is None
+    assert n.matmul_epilogue_backward(t, t, t, 2, None, None, True, True, True) is None
+    assert n.newton_schulz(t, -1, 1.0, 1.0, 1.0, 1e-7, None) is None
+    assert n.newton_schulz(t.half(), 5, 1.0, 1.0, 1.0, 1e-7, None) is None
+
+
+def test_a_library_error_is_raised_by_either(gpu, monkeypatch):
+    import torch
+
+    import kernel_library as kl
+
+    # An operand past 4 GiB is refused by the library, before a launch.
+    lhs = torch.empty(1, 1, dtype=torch.bfloat16, device=gpu)
+    wide = torch.empty(1, 2**31 - 8, dtype=torch.bfloat16, device=gpu)
+    out = torch.empty(1, 2**31 - 8, dtype=torch.bfloat16, device=gpu)
+    kl.layer_norm(lhs)
+    for _ in range(2):
+        with pytest.raises(kl.epilogue._lib.KernelLibraryError, match="32-bit"):
+            kl.matmul_epilogue(lhs, wide, out=out)
