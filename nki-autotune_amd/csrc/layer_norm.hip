@@ -26,97 +26,79 @@ size_t span(long long rows, long long ld, int D, size_t elem) {
   return rows > 0 ? ((size_t)(rows - 1) * (size_t)ld + (size_t)D) * elem : 0;
 }
 
-// Every row of p starts on 16 bytes (or there is no p).
-bool rows_16(const void* p, long long ld, size_t elem) {
-  return !p || ((uintptr_t)p % 16 == 0 && (size_t)ld * elem % 16 == 0);
-}
-
 int launched(const char* what) {
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? MI_OK : fail(-(int)e, "%s: %s", what, hipGetErrorString(e));
 }
 
-template <class T, int VW, int E, int WPR>
+// Threads of a block, and as many blocks as the chip holds with the rows'
+// values, parameters and next row in registers: each walks over the rows.
+template <class T, int E, int L>
 void fwd(const LnFwd& p, hipStream_t s) {
-  constexpr int RPB = WPR == 1 ? 4 : 1;
-  const long long blocks = (p.rows + RPB - 1) / RPB;
-  mi::layer_norm_kernel<T, VW, E, WPR>
-      <<<dim3((unsigned)(blocks < kMaxGrid ? blocks : kMaxGrid)), dim3(WPR == 1 ? 256 : WPR * 64), 0, s>>>(p);
-}
-
-template <class T, int VW>
-void fwd_pick(const LnFwd& p, hipStream_t s) {
-  const int D = p.D;
-  if (D <= 512) fwd<T, VW, 8, 1>(p, s);
-  else if (D <= 1024) fwd<T, VW, 16, 1>(p, s);
-  else if (D <= 2048) fwd<T, VW, 8, 4>(p, s);
-  else if (D <= 4096) fwd<T, VW, 16, 4>(p, s);
-  else if (VW == 1 && D <= 8192) fwd<T, 1, 8, 16>(p, s);
-  else if (VW > 1 && D <= 8192) fwd<T, 16 / sizeof(T), 32, 4>(p, s);
-  else if (VW > 1 && D <= 16384) fwd<T, 16 / sizeof(T), 16, 16>(p, s);
-  else if (VW > 1 && D <= 32768) fwd<T, 16 / sizeof(T), 32, 16>(p, s);
-  else mi::layer_norm_long_kernel<T><<<dim3((unsigned)(p.rows < kMaxGrid ? p.rows : kMaxGrid)), dim3(1024), 0, s>>>(p);
+  constexpr int ROWS = L <= 64 ? 256 / L : 1, PER_CU = L <= 256 ? 4 : 1024 / L;
+  const long long need = (p.rows + ROWS - 1) / ROWS, most = (long long)mi::capi::device_cus() * PER_CU;
+  const dim3 grid((unsigned)(need < most ? need : most)), block(ROWS * L);
+  if (p.D == E * L) mi::layer_norm_kernel<T, E, L, ROWS, true><<<grid, block, 0, s>>>(p);
+  else mi::layer_norm_kernel<T, E, L, ROWS, false><<<grid, block, 0, s>>>(p);
 }
 
 template <class T>
-void fwd_run(const LnFwd& p, bool vec, hipStream_t s) {
-  if (vec) fwd_pick<T, 16 / sizeof(T)>(p, s);
-  else fwd_pick<T, 1>(p, s);
+void fwd_run(const LnFwd& p, hipStream_t s) {
+  const int D = p.D, V = 16 / (int)sizeof(T);
+  const unsigned rows = (unsigned)(p.rows < kMaxGrid ? p.rows : kMaxGrid);
+  if (D < V) mi::layer_norm_long_kernel<T, 64><<<dim3(rows), dim3(64), 0, s>>>(p);
+  else if (D <= 128) fwd<T, 8, 16>(p, s);
+  else if (D <= 512) fwd<T, 8, 64>(p, s);
+  else if (D <= 1024) fwd<T, 16, 64>(p, s);
+  else if (D <= 2048) fwd<T, 8, 256>(p, s);
+  else if (D <= 4096) fwd<T, 16, 256>(p, s);
+  else if (D <= 8192) fwd<T, 16, 512>(p, s);
+  else if (D <= 16384) fwd<T, 16, 1024>(p, s);
+  else mi::layer_norm_long_kernel<T, 1024><<<dim3(rows), dim3(1024), 0, s>>>(p);
 }
 
-// Blocks of the gradient's kernel: each leaves a row of partial sums.
+// Rows longer than this, or shorter than 16 bytes, are read more than once.
+int bwd_most(int dtype) { return dtype == MI_DTYPE_F32 ? 8192 : 16384; }
+
+// Lanes of a row and blocks of the gradient's kernel; each block leaves a row
+// of partial sums.
 struct BwdPlan {
-  int rows_per_block, blocks;
+  int lanes, blocks;
   bool is_long;
 };
-BwdPlan bwd_plan(long long rows, int D, int dtype, bool vec) {
+BwdPlan bwd_plan(long long rows, int D, int dtype) {
   BwdPlan b;
-  b.is_long = D > (vec ? 16384 : 8192);
-  b.rows_per_block = D <= (vec && dtype == MI_DTYPE_BF16 ? 4096 : 2048) ? 8 : 1;
-  const long long most = b.is_long ? kLongChunks : b.rows_per_block == 8 ? 256 : 512;
-  const long long need = (rows + b.rows_per_block - 1) / b.rows_per_block;
+  const bool f32 = dtype == MI_DTYPE_F32;
+  b.is_long = D > bwd_most(dtype) || D < (f32 ? 4 : 8);
+  b.lanes = D <= 128 ? 16 : D <= 512 ? 64 : D <= 2048 ? 256 : D <= 4096 ? 512 : 1024;
+  const int per_block = b.is_long ? 1 : 1024 / b.lanes;
+  const long long need = (rows + per_block - 1) / per_block, most = b.is_long ? kLongChunks : mi::capi::device_cus();
   b.blocks = (int)(need < most ? (need > 0 ? need : 1) : most);
   return b;
 }
 
-template <class T, int VW, int E, int WPR>
+template <class T, int E, int L>
 void bwd(const LnBwd& p, const BwdPlan& b, hipStream_t s) {
-  constexpr int WAVES = WPR == 1 ? 8 : WPR;
-  mi::layer_norm_bwd_kernel<T, VW, E, WPR, WAVES><<<dim3((unsigned)b.blocks), dim3(WAVES * 64), 0, s>>>(p);
-}
-
-template <class T, int VW>
-void bwd_pick(const LnBwd& p, const BwdPlan& b, hipStream_t s) {
-  const int D = p.D;
-  if (b.is_long) {
-    if (p.dx)
-      mi::layer_norm_bwd_long_kernel<T><<<dim3((unsigned)(p.rows < kMaxGrid ? p.rows : kMaxGrid)), dim3(1024), 0, s>>>(p);
-    if (p.part)
-      mi::layer_norm_columns_kernel<T><<<dim3((unsigned)((D + 255) / 256), (unsigned)b.blocks), dim3(256), 0, s>>>(p);
-  } else if (b.rows_per_block == 8) {
-    if (D <= 512) bwd<T, VW, 8, 1>(p, b, s);
-    else if (D <= 1024) bwd<T, VW, 16, 1>(p, b, s);
-    else if (D <= 2048) bwd<T, VW, 32, 1>(p, b, s);
-    else if constexpr (VW > 1 && std::is_same_v<T, Bf16>) bwd<T, VW, 64, 1>(p, b, s);
-  } else {
-    if (D <= 4096) {
-      if constexpr (VW == 1 || !std::is_same_v<T, Bf16>) bwd<T, VW, 8, 8>(p, b, s);
-    } else if (D <= 8192) bwd<T, VW, 16, 8>(p, b, s);
-    else if constexpr (VW > 1) bwd<T, VW, 32, 8>(p, b, s);
-  }
+  const dim3 grid((unsigned)b.blocks), block(1024);
+  if (p.D == E * L) mi::layer_norm_bwd_kernel<T, E, L, 1024 / L, true><<<grid, block, 0, s>>>(p);
+  else mi::layer_norm_bwd_kernel<T, E, L, 1024 / L, false><<<grid, block, 0, s>>>(p);
 }
 
 template <class T>
-void bwd_run(const LnBwd& p, const BwdPlan& b, bool vec, hipStream_t s) {
-  if (vec) bwd_pick<T, 16 / sizeof(T)>(p, b, s);
-  else bwd_pick<T, 1>(p, b, s);
-}
-
-// Whether every row of the gradient's operands can be read 16 bytes at a time.
-bool bwd_vec(const mi_layer_norm_grad_args* a) {
-  const size_t es = elem_size(a->dtype), ps = a->params_f32 ? 4 : es;
-  return rows_16(a->x, a->ldx, es) && rows_16(a->dout, a->lddout, es) && rows_16(a->dx, a->D, es) &&
-         rows_16(a->weight, 0, ps) && (size_t)a->D * es % 16 == 0;
+void bwd_run(const LnBwd& p, const BwdPlan& b, hipStream_t s) {
+  const int D = p.D;
+  if (b.is_long) {
+    const unsigned rows = (unsigned)(p.rows < kMaxGrid ? p.rows : kMaxGrid);
+    if (p.dx && D < 64) mi::layer_norm_bwd_long_kernel<T, 64><<<dim3(rows), dim3(64), 0, s>>>(p);
+    else if (p.dx) mi::layer_norm_bwd_long_kernel<T, 1024><<<dim3(rows), dim3(1024), 0, s>>>(p);
+    if (p.part)
+      mi::layer_norm_columns_kernel<T><<<dim3((unsigned)((D + 255) / 256), (unsigned)b.blocks), dim3(256), 0, s>>>(p);
+  } else if (D <= 128) bwd<T, 8, 16>(p, b, s);
+  else if (D <= 512) bwd<T, 8, 64>(p, b, s);
+  else if (D <= 2048) bwd<T, 8, 256>(p, b, s);
+  else if (D <= 4096) bwd<T, 8, 512>(p, b, s);
+  else if (D <= 8192) bwd<T, 8, 1024>(p, b, s);
+  else if constexpr (sizeof(T) == 2) bwd<T, 16, 1024>(p, b, s);
 }
 
 int check_common(long long rows, int D, long long ldx, int dtype) {
@@ -148,12 +130,10 @@ int mi_layer_norm(const mi_layer_norm_args* a, void* stream) {
       overlap(a->y, yb, a->bias, D * ps) || overlap(a->y, yb, a->mean, sb) || overlap(a->y, yb, a->rstd, sb))
     return fail(MI_E_ARGS, "y overlaps another operand");
   const LnFwd p = {a->x, a->weight, a->bias, a->y, a->mean, a->rstd, a->rows, a->ldx, a->D, a->eps, a->params_f32 != 0};
-  const bool vec = rows_16(a->x, a->ldx, es) && rows_16(a->y, a->D, es) && rows_16(a->weight, 0, ps) &&
-                   rows_16(a->bias, 0, ps);
   const hipStream_t s = (hipStream_t)stream;
-  if (a->dtype == MI_DTYPE_BF16) fwd_run<Bf16>(p, vec, s);
-  else if (a->dtype == MI_DTYPE_F16) fwd_run<Fp16>(p, vec, s);
-  else fwd_run<float>(p, vec, s);
+  if (a->dtype == MI_DTYPE_BF16) fwd_run<Bf16>(p, s);
+  else if (a->dtype == MI_DTYPE_F16) fwd_run<Fp16>(p, s);
+  else fwd_run<float>(p, s);
   return launched("layer norm");
 }
 
@@ -161,8 +141,8 @@ int mi_layer_norm_backward_workspace(const mi_layer_norm_grad_args* a, unsigned 
   if (!a || !bytes) return fail(MI_E_ARGS, "null arguments");
   const int rc = check_common(a->rows, a->D, a->ldx, a->dtype);
   if (rc != MI_OK) return rc;
-  const BwdPlan b = bwd_plan(a->rows, a->D, a->dtype, bwd_vec(a));
-  *bytes = a->dweight || a->dbias ? 2ull * (unsigned long long)b.blocks * (unsigned long long)a->D * 4ull : 0ull;
+  const BwdPlan b = bwd_plan(a->rows, a->D, a->dtype);
+  *bytes = a->rows > 0 && (a->dweight || a->dbias) ? 2ull * (unsigned long long)b.blocks * (unsigned long long)a->D * 4ull : 0ull;
   return MI_OK;
 }
 
@@ -196,15 +176,25 @@ int mi_layer_norm_backward(const mi_layer_norm_grad_args* a, void* workspace, un
     for (int j = 0; j < i; ++j)
       if (overlap(out[i].p, out[i].n, out[j].p, out[j].n)) return fail(MI_E_ARGS, "two outputs overlap");
   }
-  const bool f32 = a->dtype == MI_DTYPE_F32;
-  const bool vec = bwd_vec(a);
-  const BwdPlan b = bwd_plan(a->rows, a->D, a->dtype, vec);
-  const LnBwd p = {a->dout, a->x,         a->weight, a->mean, a->rstd, a->rows > 0 ? a->dx : nullptr, need ? (float*)workspace : nullptr,
-                   a->rows, a->lddout, a->ldx,    a->D,    a->params_f32 != 0};
   const hipStream_t s = (hipStream_t)stream;
-  if (a->dtype == MI_DTYPE_BF16) bwd_run<Bf16>(p, b, vec, s);
-  else if (a->dtype == MI_DTYPE_F16) bwd_run<Fp16>(p, b, vec, s);
-  else bwd_run<float>(p, b, vec, s);
+  if (a->rows == 0) {
+    // No row to read (the kernels take at least one): the sums are 0.
+    for (void* g : {a->dweight, a->dbias}) {
+      if (!g) continue;
+      const size_t n = D * ps / 2;
+      mi::fill_zero_kernel<<<dim3((unsigned)((n + 255) / 256 < 1024 ? (n + 255) / 256 : 1024)), dim3(256), 0, s>>>((uint16_t*)g, n);
+      const int zrc = launched("zero gradient");
+      if (zrc != MI_OK) return zrc;
+    }
+    return MI_OK;
+  }
+  const bool f32 = a->dtype == MI_DTYPE_F32;
+  const BwdPlan b = bwd_plan(a->rows, a->D, a->dtype);
+  const LnBwd p = {a->dout, a->x,         a->weight, a->mean, a->rstd, a->dx, need ? (float*)workspace : nullptr,
+                   a->rows, a->lddout, a->ldx,    a->D,    a->params_f32 != 0};
+  if (a->dtype == MI_DTYPE_BF16) bwd_run<Bf16>(p, b, s);
+  else if (a->dtype == MI_DTYPE_F16) bwd_run<Fp16>(p, b, s);
+  else bwd_run<float>(p, b, s);
   const int lrc = launched("layer norm gradient");
   if (lrc != MI_OK || !need) return lrc;
   const ColumnSum c = {(const float*)workspace, {a->dweight, a->dbias}, b.blocks, a->D};

@@ -12,15 +12,21 @@
 //
 // Both passes read every row once: its E values per lane stay in registers
 // between the sums and the output, so the bytes that cross HBM are the
-// tensors' own.  A row belongs to WPR waves (WPR * 64 lanes of E values).
-// The gradient's blocks walk over many rows and keep the column sums of
-// dweight and dbias in registers too (2 * E per lane); each block writes one
-// row of partial sums, and column_sum_kernel adds those in block order.
+// tensors' own.  A row belongs to L lanes (16 of a wave, a wave, or up to 16
+// waves).  Blocks walk over the rows with the parameters in registers and the
+// next row's loads in flight behind this row's work; the gradient's keep the
+// column sums of dweight and dbias in registers too (2 E a lane), add their
+// rows' through LDS at the end, and each leaves one row of partial sums, which
+// column_sum_kernel adds in block order.
 //
-// x, dout: bf16, fp16 or fp32 (T); weight and bias: T or fp32 (a run-time
-// flag: a wave-uniform branch per group of loads).  VW consecutive values
-// per load: 16 bytes (8, or 4 of fp32) where every row starts on 16 bytes,
-// else 1, lanes next to each other either way.
+// Every load and store is 16 bytes (8 values, 4 of fp32), aligned or not (the
+// hardware takes any address), and none is in a branch: a wait for a load
+// would otherwise wait for all of them.  Where a lane's values would pass the
+// row's end, it takes the row's last 16 bytes, computes what the lanes that
+// own them compute, stores the same, and leaves them out of the row's sums;
+// rows past the last are the last one again, left out of the column sums.
+// Measured on one MI355X against a copy's 4.9 TB/s: see the launches in
+// layer_norm.hip.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <hip/hip_fp16.h>
@@ -50,50 +56,42 @@ __device__ __forceinline__ Bf16 from_f32<Bf16>(float x) { return Bf16{__builtin_
 template <>
 __device__ __forceinline__ Fp16 from_f32<Fp16>(float x) { return Fp16{__builtin_bit_cast(uint16_t, (_Float16)x)}; }
 
-// V consecutive values: one access where they fill 16 (or, fp32 by 8, 32)
-// bytes.
-template <class T, int V>
-struct alignas(V * sizeof(T) < 16 ? V * sizeof(T) : 16) Pack {
+// 16 bytes of consecutive values at any address.
+template <class T>
+struct __attribute__((packed, aligned(sizeof(T)))) Pack {
+  static constexpr int V = 16 / sizeof(T);
   T v[V];
 };
-template <class T, int V>
-__device__ __forceinline__ void load_f32(const T* __restrict__ p, float (&out)[V]) {
-  const Pack<T, V> x = *(const Pack<T, V>*)p;
-#pragma unroll
-  for (int i = 0; i < V; ++i) out[i] = to_f32(x.v[i]);
+template <class T>
+__device__ __forceinline__ Pack<T> load_pack(const T* p) {
+  return *(const Pack<T>*)p;
 }
-template <class T, int V>
-__device__ __forceinline__ void store_f32(T* __restrict__ p, const float (&in)[V]) {
-  Pack<T, V> x;
+template <class T>
+__device__ __forceinline__ void store_pack(T* p, const float (&in)[Pack<T>::V]) {
+  Pack<T> x;
 #pragma unroll
-  for (int i = 0; i < V; ++i) x.v[i] = from_f32<T>(in[i]);
-  *(Pack<T, V>*)p = x;
+  for (int i = 0; i < Pack<T>::V; ++i) x.v[i] = from_f32<T>(in[i]);
+  *(Pack<T>*)p = x;
 }
-// A row of parameters: T, or fp32 where `f32`.
-template <class T, int V>
-__device__ __forceinline__ void load_param(const void* p, bool f32, size_t at, float (&out)[V]) {
-  if (f32) load_f32<float, V>((const float*)p + at, out);
-  else load_f32<T, V>((const T*)p + at, out);
+// A row of parameters: T, or fp32 where `f32`; `other` where there is none.
+template <class T>
+__device__ __forceinline__ float param_at(const void* p, bool f32, size_t at, float other) {
+  return !p ? other : f32 ? ((const float*)p)[at] : to_f32(((const T*)p)[at]);
 }
 
-template <int V>
-__device__ __forceinline__ void fill(float (&x)[V], float to) {
-#pragma unroll
-  for (int i = 0; i < V; ++i) x[i] = to;
-}
-
-// Sums a and b over the WPR waves of a row: every lane gets both.  `turn`
+// Sums a and b over the L lanes of a row: every lane gets both.  `turn`
 // counts the calls: with more than one wave the sums cross LDS in two places
-// used by turns, so one barrier a call is enough (a wave can only be one
-// call ahead of the others).
-template <int WPR>
-__device__ __forceinline__ void row_sum2(float& a, float& b, float (*xs)[WPR][2], int wave, int lane, int& turn) {
+// used by turns, so one barrier a call is enough (a wave can only be one call
+// ahead of the others).  wave: within the row.
+template <int L>
+__device__ __forceinline__ void row_sum2(float& a, float& b, float (*xs)[L < 64 ? 1 : L / 64][2], int wave, int lane,
+                                         int& turn) {
 #pragma unroll
-  for (int s = 32; s > 0; s >>= 1) {
+  for (int s = (L < 64 ? L : 64) / 2; s > 0; s >>= 1) {
     a += __shfl_xor(a, s);
     b += __shfl_xor(b, s);
   }
-  if constexpr (WPR > 1) {
+  if constexpr (L > 64) {
     if (lane == 0) {
       xs[turn & 1][wave][0] = a;
       xs[turn & 1][wave][1] = b;
@@ -102,7 +100,7 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, float (*xs)[WPR][2]
     a = 0.0f;
     b = 0.0f;
 #pragma unroll
-    for (int w = 0; w < WPR; ++w) {
+    for (int w = 0; w < L / 64; ++w) {
       a += xs[turn & 1][w][0];
       b += xs[turn & 1][w][1];
     }
@@ -116,6 +114,22 @@ __device__ __forceinline__ float norm_rstd(float var, float eps) {
   return 1.0f / __builtin_sqrtf((var < 0.0f ? 0.0f : var) + eps);
 }
 
+// Where a lane's packs of a row lie, and which of their values are its own.
+template <int V, int G, int L, bool EXACT>
+struct RowSplit {
+  int at[G];   // first element of pack g
+  int own[G];  // its own are elements own[g] .. V - 1 of it
+  __device__ __forceinline__ void init(int in_row, int D) {
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const int d = (g * L + in_row) * V;
+      at[g] = EXACT || d + V <= D ? d : D - V;
+      own[g] = EXACT ? 0 : d - at[g];
+    }
+  }
+  __device__ __forceinline__ float mine(int g, int i, float x) const { return EXACT || i >= own[g] ? x : 0.0f; }
+};
+
 struct LnFwd {
   const void *x, *weight, *bias;  // weight, bias: NULL for 1 and 0
   void* y;
@@ -126,98 +140,108 @@ struct LnFwd {
   bool params_f32;
 };
 
-// WPR == 1: blocks of 4 waves, a row each; otherwise a block per row.
-template <class T, int VW, int E, int WPR>
-__global__ __launch_bounds__(WPR == 1 ? 256 : WPR * 64) void layer_norm_kernel(const LnFwd p) {
-  constexpr int G = E / VW, RPB = WPR == 1 ? 4 : 1;
-  __shared__ float xs[2][WPR][2];
-  const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int in_row = WPR == 1 ? lane : tid;
+// GROUPS rows at a time in a block of GROUPS * L threads.  EXACT: D = E * L.
+template <class T, int E, int L, int GROUPS, bool EXACT>
+__global__ __launch_bounds__(L* GROUPS) void layer_norm_kernel(const LnFwd p) {
+  constexpr int V = Pack<T>::V, G = E / V;
+  static_assert(L <= 64 || GROUPS == 1, "rows of several waves have their block to themselves");
+  __shared__ float xs[2][L < 64 ? 1 : L / 64][2];
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int in_row = tid % L;
   const float inv_d = 1.0f / (float)p.D;
-  int turn = 0;
-  for (long long r = (long long)blockIdx.x * RPB + (WPR == 1 ? wave : 0); r < p.rows; r += (long long)gridDim.x * RPB) {
-    const T* x = (const T*)p.x + (size_t)r * (size_t)p.ldx;
-    float v[G][VW];
-    float sum = 0.0f, none = 0.0f;
+  RowSplit<V, G, L, EXACT> split;
+  split.init(in_row, p.D);
+  const auto row_of = [&](long long r) { return r < p.rows ? r : p.rows - 1; };
+  const long long step = (long long)gridDim.x * GROUPS;
+  long long r = (long long)blockIdx.x * GROUPS + tid / L;
+  Pack<T> next[G];
+  const auto fetch = [&](long long at) __attribute__((always_inline)) {
+    const T* x = (const T*)p.x + (size_t)at * (size_t)p.ldx;
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      const int d = (g * WPR * 64 + in_row) * VW;
-      if (d < p.D) load_f32<T, VW>(x + d, v[g]);
-      else fill(v[g], 0.0f);
+    for (int g = 0; g < G; ++g) next[g] = load_pack(x + split.at[g]);
+  };
+  fetch(row_of(r));
+  float w[G][V], b[G][V];
+#pragma unroll
+  for (int g = 0; g < G; ++g)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      w[g][i] = param_at<T>(p.weight, p.params_f32, split.at[g] + i, 1.0f);
+      b[g][i] = param_at<T>(p.bias, p.params_f32, split.at[g] + i, 0.0f);
     }
+  int turn = 0;
+  for (long long first = (long long)blockIdx.x * GROUPS; first < p.rows; first += step, r += step) {
+    float v[G][V];
 #pragma unroll
     for (int g = 0; g < G; ++g)
 #pragma unroll
-      for (int i = 0; i < VW; ++i) sum += v[g][i];
-    row_sum2<WPR>(sum, none, xs, wave, lane, turn);
+      for (int i = 0; i < V; ++i) v[g][i] = to_f32(next[g].v[i]);
+    fetch(row_of(r + step));
+    float sum = 0.0f, none = 0.0f;
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int i = 0; i < V; ++i) sum += split.mine(g, i, v[g][i]);
+    row_sum2<L>(sum, none, xs, wave, lane, turn);
     float mean = sum * inv_d;
     // The centred values' own sum is what rounding left in the mean: taken
     // out again, so rows far from zero keep their digits.
     float rest = 0.0f, sq = 0.0f;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      const bool in = (g * WPR * 64 + in_row) * VW < p.D;
 #pragma unroll
-      for (int i = 0; i < VW; ++i) {
-        v[g][i] = in ? v[g][i] - mean : 0.0f;
-        rest += v[g][i];
-        sq += v[g][i] * (v[g][i] * inv_d);  // a share of the mean each: the sum stays in range wherever the variance does
+      for (int i = 0; i < V; ++i) {
+        v[g][i] -= mean;
+        const float c = split.mine(g, i, v[g][i]);
+        rest += c;
+        sq += c * (c * inv_d);  // a share of the mean each: the sum stays in range wherever the variance does
       }
     }
-    row_sum2<WPR>(rest, sq, xs, wave, lane, turn);
+    row_sum2<L>(rest, sq, xs, wave, lane, turn);
     rest *= inv_d;
     mean += rest;
     const float rstd = norm_rstd(sq - rest * rest, p.eps);
-    T* y = (T*)p.y + (size_t)r * (size_t)p.D;
+    T* y = (T*)p.y + (size_t)row_of(r) * (size_t)p.D;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      const int d = (g * WPR * 64 + in_row) * VW;
-      if (d >= p.D) continue;
-      float w[VW], b[VW], o[VW];
-      if (p.weight) load_param<T, VW>(p.weight, p.params_f32, d, w);
-      else fill(w, 1.0f);
-      if (p.bias) load_param<T, VW>(p.bias, p.params_f32, d, b);
-      else fill(b, 0.0f);
+      float o[V];
 #pragma unroll
-      for (int i = 0; i < VW; ++i) o[i] = (v[g][i] - rest) * rstd * w[i] + b[i];
-      store_f32<T, VW>(y + d, o);
+      for (int i = 0; i < V; ++i) o[i] = (v[g][i] - rest) * rstd * w[g][i] + b[g][i];
+      store_pack(y + split.at[g], o);
     }
-    if (in_row == 0) {
+    if (in_row == 0 && r < p.rows) {
       if (p.mean) p.mean[r] = mean;
       if (p.rstd) p.rstd[r] = rstd;
     }
   }
 }
 
-// Rows longer than registers hold: a block of 1024 per row reads it three
-// times (from L2 after the first).
-template <class T>
-__global__ __launch_bounds__(1024) void layer_norm_long_kernel(const LnFwd p) {
-  __shared__ float xs[2][16][2];
+// Rows longer than registers hold, or shorter than 16 bytes: a block of B
+// threads per row reads it three times (from L2 after the first).
+template <class T, int B>
+__global__ __launch_bounds__(B) void layer_norm_long_kernel(const LnFwd p) {
+  __shared__ float xs[2][B / 64][2];
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const float inv_d = 1.0f / (float)p.D;
   int turn = 0;
   for (long long r = blockIdx.x; r < p.rows; r += gridDim.x) {
     const T* x = (const T*)p.x + (size_t)r * (size_t)p.ldx;
     float sum = 0.0f, none = 0.0f;
-    for (int d = tid; d < p.D; d += 1024) sum += to_f32(x[d]);
-    row_sum2<16>(sum, none, xs, wave, lane, turn);
+    for (int d = tid; d < p.D; d += B) sum += to_f32(x[d]);
+    row_sum2<B>(sum, none, xs, wave, lane, turn);
     float mean = sum * inv_d, rest = 0.0f, sq = 0.0f;
-    for (int d = tid; d < p.D; d += 1024) {
+    for (int d = tid; d < p.D; d += B) {
       const float c = to_f32(x[d]) - mean;
       rest += c;
       sq += c * (c * inv_d);
     }
-    row_sum2<16>(rest, sq, xs, wave, lane, turn);
+    row_sum2<B>(rest, sq, xs, wave, lane, turn);
     rest *= inv_d;
     const float rstd = norm_rstd(sq - rest * rest, p.eps);
     T* y = (T*)p.y + (size_t)r * (size_t)p.D;
-    for (int d = tid; d < p.D; d += 1024) {
-      float w[1] = {1.0f}, b[1] = {0.0f};
-      if (p.weight) load_param<T, 1>(p.weight, p.params_f32, d, w);
-      if (p.bias) load_param<T, 1>(p.bias, p.params_f32, d, b);
-      y[d] = from_f32<T>((to_f32(x[d]) - mean - rest) * rstd * w[0] + b[0]);
-    }
+    for (int d = tid; d < p.D; d += B)
+      y[d] = from_f32<T>((to_f32(x[d]) - mean - rest) * rstd * param_at<T>(p.weight, p.params_f32, d, 1.0f) +
+                         param_at<T>(p.bias, p.params_f32, d, 0.0f));
     if (tid == 0) {
       if (p.mean) p.mean[r] = mean + rest;
       if (p.rstd) p.rstd[r] = rstd;
@@ -235,112 +259,121 @@ struct LnBwd {
   bool weight_f32;
 };
 
-// WAVES waves a block, WPR of them to a row.
-template <class T, int VW, int E, int WPR, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void layer_norm_bwd_kernel(const LnBwd p) {
-  constexpr int G = E / VW, RPB = WAVES / WPR;
-  static_assert(WPR == 1 || RPB == 1, "a block holds single-wave rows or one row");
-  __shared__ float xs[2][WPR][2];
-  const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int in_row = WPR == 1 ? lane : tid;
+// GROUPS rows at a time in a block of GROUPS * L threads.  EXACT: D = E * L.
+template <class T, int E, int L, int GROUPS, bool EXACT>
+__global__ __launch_bounds__(L* GROUPS) void layer_norm_bwd_kernel(const LnBwd p) {
+  constexpr int V = Pack<T>::V, G = E / V, WPR = L < 64 ? 1 : L / 64;
+  __shared__ float xs[GROUPS][2][WPR][2];
+  __shared__ float cols[GROUPS > 1 ? GROUPS : 1][GROUPS > 1 ? L * V : 1];
+  const int tid = (int)threadIdx.x, lane = tid & 63;
+  const int in_row = tid % L, group = tid / L, wave = in_row >> 6;
   const float inv_d = 1.0f / (float)p.D;
-  float dw[G][VW], db[G][VW];
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
-    fill(dw[g], 0.0f);
-    fill(db[g], 0.0f);
-  }
-  int turn = 0;
-  for (long long r = (long long)blockIdx.x * RPB + (WPR == 1 ? wave : 0); r < p.rows; r += (long long)gridDim.x * RPB) {
-    const T* x = (const T*)p.x + (size_t)r * (size_t)p.ldx;
-    const T* dout = (const T*)p.dout + (size_t)r * (size_t)p.lddout;
-    const float mean = p.mean[r], rstd = p.rstd[r];
-    Pack<T, VW> xv[G], dv[G];
+  RowSplit<V, G, L, EXACT> split;
+  split.init(in_row, p.D);
+  const auto row_of = [&](long long r) { return r < p.rows ? r : p.rows - 1; };
+  const long long step = (long long)gridDim.x * GROUPS;
+  long long r = (long long)blockIdx.x * GROUPS + group;
+  Pack<T> nx[G], nd[G];
+  float nmean, nrstd;
+  const auto fetch = [&](long long at) __attribute__((always_inline)) {
+    const T* x = (const T*)p.x + (size_t)at * (size_t)p.ldx;
+    const T* dout = (const T*)p.dout + (size_t)at * (size_t)p.lddout;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      const int d = (g * WPR * 64 + in_row) * VW;
-      if (d < p.D) {
-        xv[g] = *(const Pack<T, VW>*)(x + d);
-        dv[g] = *(const Pack<T, VW>*)(dout + d);
-      }
+      nx[g] = load_pack(x + split.at[g]);
+      nd[g] = load_pack(dout + split.at[g]);
     }
+    nmean = p.mean[at];
+    nrstd = p.rstd[at];
+  };
+  fetch(row_of(r));
+  float w[G][V], dw[G][V], db[G][V];
+#pragma unroll
+  for (int g = 0; g < G; ++g)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      w[g][i] = param_at<T>(p.weight, p.weight_f32, split.at[g] + i, 1.0f);
+      dw[g][i] = 0.0f;
+      db[g][i] = 0.0f;
+    }
+  int turn = 0;
+  for (long long first = (long long)blockIdx.x * GROUPS; first < p.rows; first += step, r += step) {
+    Pack<T> xv[G], dv[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      xv[g] = nx[g];
+      dv[g] = nd[g];
+    }
+    const float mean = nmean, rstd = nrstd;
+    fetch(row_of(r + step));
+    const bool live = r < p.rows;
     float sg = 0.0f, sgx = 0.0f;
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      const int d = (g * WPR * 64 + in_row) * VW;
-      if (d >= p.D) continue;
-      float w[VW];
-      if (p.weight) load_param<T, VW>(p.weight, p.weight_f32, d, w);
-      else fill(w, 1.0f);
+    for (int g = 0; g < G; ++g)
 #pragma unroll
-      for (int i = 0; i < VW; ++i) {
+      for (int i = 0; i < V; ++i) {
         const float dy = to_f32(dv[g].v[i]), xh = (to_f32(xv[g].v[i]) - mean) * rstd;
-        dw[g][i] += dy * xh;
-        db[g][i] += dy;
-        sg += dy * w[i];
-        sgx += dy * w[i] * xh;
+        const float counted = live ? dy : 0.0f;
+        dw[g][i] += live ? dy * xh : 0.0f;
+        db[g][i] += counted;
+        const float gw = split.mine(g, i, dy * w[g][i]);
+        sg += gw;
+        sgx += split.mine(g, i, gw * xh);
       }
-    }
     if (!p.dx) continue;
-    row_sum2<WPR>(sg, sgx, xs, wave, lane, turn);
+    row_sum2<L>(sg, sgx, xs[group], wave, lane, turn);
     sg *= inv_d;
     sgx *= inv_d;
-    T* dx = (T*)p.dx + (size_t)r * (size_t)p.D;
+    T* dx = (T*)p.dx + (size_t)row_of(r) * (size_t)p.D;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      const int d = (g * WPR * 64 + in_row) * VW;
-      if (d >= p.D) continue;
-      float w[VW], o[VW];
-      if (p.weight) load_param<T, VW>(p.weight, p.weight_f32, d, w);
-      else fill(w, 1.0f);
+      float o[V];
 #pragma unroll
-      for (int i = 0; i < VW; ++i) {
+      for (int i = 0; i < V; ++i) {
         const float xh = (to_f32(xv[g].v[i]) - mean) * rstd;
-        o[i] = rstd * (to_f32(dv[g].v[i]) * w[i] - sg - xh * sgx);
+        o[i] = rstd * (to_f32(dv[g].v[i]) * w[g][i] - sg - xh * sgx);
       }
-      store_f32<T, VW>(dx + d, o);
+      store_pack(dx + split.at[g], o);
     }
   }
   if (!p.part) return;
   float* part_w = p.part + (size_t)blockIdx.x * (size_t)p.D;
   float* part_b = part_w + (size_t)gridDim.x * (size_t)p.D;
-  if constexpr (RPB == 1) {
+  if constexpr (GROUPS == 1) {
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      const int d = (g * WPR * 64 + in_row) * VW;
-      if (d >= p.D) continue;
-      store_f32<float, VW>(part_w + d, dw[g]);
-      store_f32<float, VW>(part_b + d, db[g]);
-    }
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        part_w[split.at[g] + i] = dw[g][i];
+        part_b[split.at[g] + i] = db[g][i];
+      }
   } else {
-    // The waves' sums, in wave order: one group of columns at a time in LDS.
-    __shared__ __attribute__((aligned(16))) float ws[RPB][64 * VW + 4];
-    for (int k = 0; k < 2; ++k) {
+    // The groups' sums in their order, one pack of columns at a time.
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        if (g * 64 * VW >= p.D) break;
+        if (g * L * V >= p.D) break;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < VW; ++i) ws[wave][lane * VW + i] = k ? db[g][i] : dw[g][i];
+        for (int i = 0; i < V; ++i) cols[group][in_row * V + i] = k ? db[g][i] : dw[g][i];
         __syncthreads();
-        for (int c = tid; c < 64 * VW; c += WAVES * 64) {
-          const int d = g * 64 * VW + c;
-          if (d >= p.D) break;
-          float s = ws[0][c];
+        for (int c = tid; c < L * V; c += L * GROUPS) {
+          const int d = g * L * V + c / V * V, at = d + V <= p.D ? d : p.D - V;
+          float s = cols[0][c];
 #pragma unroll
-          for (int w = 1; w < RPB; ++w) s += ws[w][c];
-          (k ? part_b : part_w)[d] = s;
+          for (int q = 1; q < GROUPS; ++q) s += cols[q][c];
+          (k ? part_b : part_w)[at + c % V] = s;
         }
       }
-    }
   }
 }
 
-// Rows longer than registers hold: dx by a block per row, and the column
-// sums by layer_norm_columns_kernel.
-template <class T>
-__global__ __launch_bounds__(1024) void layer_norm_bwd_long_kernel(const LnBwd p) {
-  __shared__ float xs[2][16][2];
+// Rows longer than registers hold, or shorter than 16 bytes: dx by a block of
+// B threads per row, and the column sums by layer_norm_columns_kernel.
+template <class T, int B>
+__global__ __launch_bounds__(B) void layer_norm_bwd_long_kernel(const LnBwd p) {
+  __shared__ float xs[2][B / 64][2];
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const float inv_d = 1.0f / (float)p.D;
   int turn = 0;
@@ -349,22 +382,18 @@ __global__ __launch_bounds__(1024) void layer_norm_bwd_long_kernel(const LnBwd p
     const T* dout = (const T*)p.dout + (size_t)r * (size_t)p.lddout;
     const float mean = p.mean[r], rstd = p.rstd[r];
     float sg = 0.0f, sgx = 0.0f;
-    for (int d = tid; d < p.D; d += 1024) {
-      float w[1] = {1.0f};
-      if (p.weight) load_param<T, 1>(p.weight, p.weight_f32, d, w);
-      const float g = to_f32(dout[d]) * w[0];
+    for (int d = tid; d < p.D; d += B) {
+      const float g = to_f32(dout[d]) * param_at<T>(p.weight, p.weight_f32, d, 1.0f);
       sg += g;
       sgx += g * ((to_f32(x[d]) - mean) * rstd);
     }
-    row_sum2<16>(sg, sgx, xs, wave, lane, turn);
+    row_sum2<B>(sg, sgx, xs, wave, lane, turn);
     sg *= inv_d;
     sgx *= inv_d;
     T* dx = (T*)p.dx + (size_t)r * (size_t)p.D;
-    for (int d = tid; d < p.D; d += 1024) {
-      float w[1] = {1.0f};
-      if (p.weight) load_param<T, 1>(p.weight, p.weight_f32, d, w);
+    for (int d = tid; d < p.D; d += B) {
       const float xh = (to_f32(x[d]) - mean) * rstd;
-      dx[d] = from_f32<T>(rstd * (to_f32(dout[d]) * w[0] - sg - xh * sgx));
+      dx[d] = from_f32<T>(rstd * (to_f32(dout[d]) * param_at<T>(p.weight, p.weight_f32, d, 1.0f) - sg - xh * sgx));
     }
   }
 }
