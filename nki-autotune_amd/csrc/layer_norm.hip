@@ -13,7 +13,7 @@ using mi::LnFwd;
 using mi::capi::fail;
 
 constexpr long long kMaxGrid = 1 << 20;  // blocks of one launch; they walk over the rows
-constexpr int kLongChunks = 64;          // row chunks of the column sums of long rows
+constexpr int kLongChunks = 256;         // row chunks of the column sums of long rows
 
 size_t elem_size(int dtype) { return dtype == MI_DTYPE_F32 ? 4 : 2; }
 
@@ -38,23 +38,26 @@ void fwd(const LnFwd& p, hipStream_t s) {
   constexpr int ROWS = L <= 64 ? 256 / L : 1, PER_CU = L <= 256 ? 4 : 1024 / L;
   const long long need = (p.rows + ROWS - 1) / ROWS, most = (long long)mi::capi::device_cus() * PER_CU;
   const dim3 grid((unsigned)(need < most ? need : most)), block(ROWS * L);
-  if (p.D == E * L) mi::layer_norm_kernel<T, E, L, ROWS, true><<<grid, block, 0, s>>>(p);
-  else mi::layer_norm_kernel<T, E, L, ROWS, false><<<grid, block, 0, s>>>(p);
+  if (p.D == E * L) mi::layer_norm_kernel<T, E, L, ROWS, true, (E < 32)><<<grid, block, 0, s>>>(p);
+  else mi::layer_norm_kernel<T, E, L, ROWS, false, (E < 32)><<<grid, block, 0, s>>>(p);
 }
 
 template <class T>
 void fwd_run(const LnFwd& p, hipStream_t s) {
-  const int D = p.D, V = 16 / (int)sizeof(T);
+  constexpr int V = 16 / (int)sizeof(T);
+  const int D = p.D;
   const unsigned rows = (unsigned)(p.rows < kMaxGrid ? p.rows : kMaxGrid);
-  if (D < V) mi::layer_norm_long_kernel<T, 64><<<dim3(rows), dim3(64), 0, s>>>(p);
+  if (D < V) mi::layer_norm_long_kernel<T, 64, 1><<<dim3(rows), dim3(64), 0, s>>>(p);
   else if (D <= 128) fwd<T, 8, 16>(p, s);
+  else if (D <= 256) fwd<T, 8, 32>(p, s);
   else if (D <= 512) fwd<T, 8, 64>(p, s);
   else if (D <= 1024) fwd<T, 16, 64>(p, s);
   else if (D <= 2048) fwd<T, 8, 256>(p, s);
   else if (D <= 4096) fwd<T, 16, 256>(p, s);
   else if (D <= 8192) fwd<T, 16, 512>(p, s);
   else if (D <= 16384) fwd<T, 16, 1024>(p, s);
-  else mi::layer_norm_long_kernel<T, 1024><<<dim3(rows), dim3(1024), 0, s>>>(p);
+  else if (D <= 32768) fwd<T, 32, 1024>(p, s);
+  else mi::layer_norm_long_kernel<T, 1024, V><<<dim3(rows), dim3(1024), 0, s>>>(p);
 }
 
 // Rows longer than this, or shorter than 16 bytes, are read more than once.
@@ -70,7 +73,7 @@ BwdPlan bwd_plan(long long rows, int D, int dtype) {
   BwdPlan b;
   const bool f32 = dtype == MI_DTYPE_F32;
   b.is_long = D > bwd_most(dtype) || D < (f32 ? 4 : 8);
-  b.lanes = D <= 128 ? 16 : D <= 512 ? 64 : D <= 2048 ? 256 : D <= 4096 ? 512 : 1024;
+  b.lanes = D <= 128 ? 16 : D <= 256 ? 32 : D <= 512 ? 64 : D <= 1024 ? 128 : D <= 2048 ? 256 : D <= 4096 ? 512 : 1024;
   const int per_block = b.is_long ? 1 : 1024 / b.lanes;
   const long long need = (rows + per_block - 1) / per_block, most = b.is_long ? kLongChunks : mi::capi::device_cus();
   b.blocks = (int)(need < most ? (need > 0 ? need : 1) : most);
@@ -89,12 +92,20 @@ void bwd_run(const LnBwd& p, const BwdPlan& b, hipStream_t s) {
   const int D = p.D;
   if (b.is_long) {
     const unsigned rows = (unsigned)(p.rows < kMaxGrid ? p.rows : kMaxGrid);
-    if (p.dx && D < 64) mi::layer_norm_bwd_long_kernel<T, 64><<<dim3(rows), dim3(64), 0, s>>>(p);
-    else if (p.dx) mi::layer_norm_bwd_long_kernel<T, 1024><<<dim3(rows), dim3(1024), 0, s>>>(p);
-    if (p.part)
-      mi::layer_norm_columns_kernel<T><<<dim3((unsigned)((D + 255) / 256), (unsigned)b.blocks), dim3(256), 0, s>>>(p);
+    constexpr int V = 16 / (int)sizeof(T);
+    const unsigned chunks = (unsigned)b.blocks;
+    if (D < V) {
+      if (p.dx) mi::layer_norm_bwd_long_kernel<T, 64, 1><<<dim3(rows), dim3(64), 0, s>>>(p);
+      if (p.part) mi::layer_norm_columns_kernel<T, 1><<<dim3(1, chunks), dim3(256), 0, s>>>(p);
+    } else {
+      if (p.dx) mi::layer_norm_bwd_long_kernel<T, 1024, V><<<dim3(rows), dim3(1024), 0, s>>>(p);
+      if (p.part)
+        mi::layer_norm_columns_kernel<T, V><<<dim3((unsigned)((D + 256 * V - 1) / (256 * V)), chunks), dim3(256), 0, s>>>(p);
+    }
   } else if (D <= 128) bwd<T, 8, 16>(p, b, s);
+  else if (D <= 256) bwd<T, 8, 32>(p, b, s);
   else if (D <= 512) bwd<T, 8, 64>(p, b, s);
+  else if (D <= 1024) bwd<T, 8, 128>(p, b, s);
   else if (D <= 2048) bwd<T, 8, 256>(p, b, s);
   else if (D <= 4096) bwd<T, 8, 512>(p, b, s);
   else if (D <= 8192) bwd<T, 8, 1024>(p, b, s);
@@ -103,6 +114,7 @@ void bwd_run(const LnBwd& p, const BwdPlan& b, hipStream_t s) {
 
 int check_common(long long rows, int D, long long ldx, int dtype) {
   if (rows < 0 || D <= 0) return fail(MI_E_ARGS, "bad size rows=%lld D=%d (D must be positive)", rows, D);
+  if (D > 1 << 30) return fail(MI_E_RANGE, "D=%d over %d", D, 1 << 30);
   if (ldx < 0) return fail(MI_E_ARGS, "negative row stride %lld", ldx);
   if (dtype != MI_DTYPE_BF16 && dtype != MI_DTYPE_F16 && dtype != MI_DTYPE_F32)
     return fail(MI_E_ARGS, "unknown dtype %d", dtype);

@@ -16,30 +16,51 @@ using mi::capi::kMaxSplit;
 
 // ---- kernels beside the products --------------------------------------
 
-// dst[r][0, cp) = src[r][0, c), then zeros: rows that start on 16 bytes.
-__global__ __launch_bounds__(256) void pad_rows_kernel(const uint16_t* __restrict__ src, uint16_t* __restrict__ dst,
-                                                       long long rows, int c, int cp) {
-  const int groups = cp / 8;
-  const long long n = rows * groups;
+// dst[r][0, cp) = src[r][0, c), then zeros: rows that start on 16 bytes.  One
+// launch for both operands of a product (blockIdx.y).
+struct PadRows {
+  const uint16_t* src;
+  uint16_t* dst;  // NULL: nothing to do
+  long long rows;
+  int c, cp;
+};
+struct PadBoth {
+  PadRows op[2];
+};
+__global__ __launch_bounds__(256) void pad_rows_kernel(const PadBoth both) {
+  const PadRows p = both.op[blockIdx.y];
+  if (!p.dst) return;
+  const int groups = p.cp / 8;
+  const long long n = p.rows * groups;
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
     const long long r = i / groups;
     const int d = (int)(i - r * groups) * 8;
-    const uint16_t* s = src + (size_t)r * (size_t)c;
-    uint32_t v[8];
+    const uint16_t* s = p.src + (size_t)r * (size_t)p.c;
+    uint16_t* t = p.dst + (size_t)r * (size_t)p.cp + d;
+    if (d + 8 <= p.c) {
+      *(mi::Pack<uint16_t>*)t = mi::load_pack(s + d);
+    } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = d + k < c ? s[d + k] : 0u;
-    *(mi::u32x4_t*)(dst + (size_t)r * (size_t)cp + d) =
-        mi::u32x4_t{v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16};
+      for (int k = 0; k < 8; ++k) t[k] = d + k < p.c ? s[d + k] : (uint16_t)0;
+    }
   }
 }
 
 // dst[r][0, c) = src[r][0, c) of rows cp apart (dst rows c apart): the way back.
 __global__ __launch_bounds__(256) void unpad_rows_kernel(const uint16_t* __restrict__ src, uint16_t* __restrict__ dst,
                                                          long long rows, int c, int cp) {
-  const long long n = rows * c;
+  const int groups = cp / 8;
+  const long long n = rows * groups;
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-    const long long r = i / c;
-    dst[i] = src[(size_t)r * (size_t)cp + (size_t)(i - r * c)];
+    const long long r = i / groups;
+    const int d = (int)(i - r * groups) * 8;
+    const uint16_t* s = src + (size_t)r * (size_t)cp + d;
+    uint16_t* t = dst + (size_t)r * (size_t)c + d;
+    if (d + 8 <= c) {
+      *(mi::Pack<uint16_t>*)t = mi::load_pack(s);
+    } else {
+      for (int k = 0; d + k < c; ++k) t[k] = s[k];
+    }
   }
 }
 
@@ -69,64 +90,78 @@ __global__ __launch_bounds__(256) void epi_sum_kernel(const float* __restrict__ 
 }
 
 // dpre[m][0, np) = bf16(dout * act'(pre)) with zeros past N, and the column
-// sums of the unrounded values over this block's rows: blockIdx.x takes 512
+// sums of the unrounded values over this block's rows: blockIdx.x takes 64 W
 // columns, the block's 4 waves rows 4 * blockIdx.y + wave, + 4 * gridDim.y, ...
+// A lane has W columns (8; 1 where N < 8); past the row's end the last W, of
+// which own .. W - 1 are its own.  Bound by its bytes: 22 us for 4096 x 4096
+// (100 MB) on one MI355X, 4.6 TB/s.
 struct ActGrad {
   const uint16_t *dout, *pre;
   uint16_t* dpre;  // NULL: not wanted
   float* part;     // [gridDim.y][N], NULL: not wanted
   int M, N, np, act;
-  bool vec;
 };
+template <int W>
 __global__ __launch_bounds__(256) void act_grad_kernel(const ActGrad p) {
-  __shared__ float xs[4][512 + 8];
+  __shared__ float xs[4][64 * W + 8];
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-  const int c = (int)blockIdx.x * 512 + lane * 8;
-  float sum[8] = {};
+  const int first = (int)blockIdx.x * 64 * W, c = first + lane * W;
+  const int at = c + W <= p.N ? c : p.N - W, own = c - at;
+  float sum[W];
+  mi::fill(sum, 0.0f);
   const int step = 4 * (int)gridDim.y;
-  auto load = [&](const uint16_t* q, int m, float (&v)[8]) __attribute__((always_inline)) {
-    const uint16_t* at = q + (size_t)m * (size_t)p.N + c;
-    if (p.vec) {
-      mi::unpack8(*(const mi::u32x4_t*)at, v);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = c + i < p.N ? mi::bf16lo((uint32_t)at[i]) : 0.0f;
-    }
-  };
   constexpr int U = 4;
-  if (c < p.np)
-    for (int m0 = 4 * (int)blockIdx.y + wave; m0 < p.M; m0 += U * step) {
-      float d[U][8], x[U][8];
+  for (int m0 = 4 * (int)blockIdx.y + wave; m0 < p.M; m0 += U * step) {
+    mi::Pack<uint16_t, W> dq[U], xq[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int m = m0 + u * step < p.M ? m0 + u * step : p.M - 1;
+      dq[u] = mi::load_pack<uint16_t, W>(p.dout + (size_t)m * (size_t)p.N + at);
+    }
+    if (p.pre) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int m = m0 + u * step;
-        if (m >= p.M) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) d[u][i] = x[u][i] = 0.0f;
-          continue;
-        }
-        load(p.dout, m, d[u]);
-        if (p.pre) load(p.pre, m, x[u]);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (p.pre)
-          mi::with_act(p.act, [&](auto a_c) __attribute__((always_inline)) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) d[u][i] *= mi::act_slope<decltype(a_c)::value>(x[u][i]);
-          });
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sum[i] += d[u][i];
-        const int m = m0 + u * step;
-        if (p.dpre && m < p.M) *(mi::u32x4_t*)(p.dpre + (size_t)m * (size_t)p.np + c) = mi::pack8(d[u]);
+        const int m = m0 + u * step < p.M ? m0 + u * step : p.M - 1;
+        xq[u] = mi::load_pack<uint16_t, W>(p.pre + (size_t)m * (size_t)p.N + at);
       }
     }
-  if (!p.part) return;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) xs[wave][lane * 8 + i] = sum[i];
+    for (int u = 0; u < U; ++u) {
+      const int m = m0 + u * step;
+      if (m >= p.M) break;
+      float d[W];
+#pragma unroll
+      for (int i = 0; i < W; ++i) d[i] = mi::bf16lo((uint32_t)dq[u].v[i]);
+      if (p.pre)
+        mi::with_act(p.act, [&](auto a_c) __attribute__((always_inline)) {
+#pragma unroll
+          for (int i = 0; i < W; ++i) d[i] *= mi::act_slope<decltype(a_c)::value>(mi::bf16lo((uint32_t)xq[u].v[i]));
+        });
+#pragma unroll
+      for (int i = 0; i < W; ++i) sum[i] += d[i];
+      if (!p.dpre || c >= p.N) continue;
+      uint16_t* row = p.dpre + (size_t)m * (size_t)p.np;
+      if (own == 0) {
+        if constexpr (W == 8) *(mi::u32x4_t*)(row + c) = mi::pack8(d);
+        else row[c] = (uint16_t)mi::pack_bf16x2(d[0], 0.0f);
+      } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+          if (i >= own) row[at + i] = (uint16_t)mi::pack_bf16x2(d[i], 0.0f);
+      }
+      if (c + W >= p.N)  // the row's last lane
+        for (int n = p.N; n < p.np; ++n) row[n] = 0;
+    }
+  }
+  if (!p.part) return;
+  if (c < p.N) {
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+      if (i >= own) xs[wave][at + i - first] = sum[i];
+  }
   __syncthreads();
-  for (int k = (int)threadIdx.x; k < 512; k += 256) {
-    const int n = (int)blockIdx.x * 512 + k;
+  for (int k = (int)threadIdx.x; k < 64 * W; k += 256) {
+    const int n = first + k;
     if (n < p.N) p.part[(size_t)blockIdx.y * (size_t)p.N + n] = ((xs[0][k] + xs[1][k]) + xs[2][k]) + xs[3][k];
   }
 }
@@ -142,6 +177,11 @@ unsigned blocks_for(long long items) {
   const long long b = (items + 255) / 256;
   return (unsigned)(b < 1 ? 1 : b > 8192 ? 8192 : b);
 }
+
+// Columns of an output whose block rows (256 of 4 bytes a column) stay within
+// 32-bit offsets with room to spare: wider ones are stored element by element
+// and not split.
+constexpr int kWide = 1 << 20;
 
 int up8(int v) { return (v + 7) / 8 * 8; }
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
@@ -200,7 +240,7 @@ mi_tile_cfg pick(int M, int N, int K, bool bt) {
     for (const int parts : {1, 2, 3, 4, 6, 8, 12, 16}) {
       const int each = (kt + parts - 1) / parts;
       // Parts of at least three K tiles, none empty, in at most four blocks a unit.
-      if (parts > 1 && (kt / parts < 3 || (parts - 1) * each >= kt || tiles * parts > 4ll * cus ||
+      if (parts > 1 && (N > kWide || kt / parts < 3 || (parts - 1) * each >= kt || tiles * parts > 4ll * cus ||
                         (double)parts * M * N * 4.0 > (double)mi::capi::kMaxWorkspace))
         break;
       const long long blocks = (tiles * parts + cus - 1) / cus, rounds = (blocks + e.per_cu - 1) / e.per_cu;
@@ -238,6 +278,7 @@ int plan(const uint16_t* a, int lda, const uint16_t* b, int ldb, long long b_row
   const long long kt = ((long long)K + c.block_k - 1) / c.block_k, each = (kt + c.split_k - 1) / c.split_k;
   if ((long long)(c.split_k - 1) * each >= kt && c.split_k > 1)
     return fail(MI_E_SPLIT, "split_k=%d leaves a K part empty at K=%d, block_k=%d", c.split_k, K, c.block_k);
+  if (c.split_k > 1 && N > kWide) return fail(MI_E_SPLIT, "split_k=%d takes at most %d columns", c.split_k, kWide);
   // Loads run up to a block past the last row and a K tile past the last column.
   const unsigned long long a_span = ((unsigned long long)M + c.block_m) * lda * 2ull + 16ull * c.block_k;
   const unsigned long long b_span = bt ? ((unsigned long long)N + c.block_n) * ldb * 2ull + 16ull * c.block_k
@@ -280,10 +321,13 @@ Padded padded(const void* p, long long rows, int c, size_t* ws) {
   }
   return q;
 }
-int pad(const void* src, char* ws, const Padded& q, long long rows, int c, hipStream_t s) {
-  if (!q.on) return MI_OK;
-  pad_rows_kernel<<<dim3(blocks_for(rows * (q.ld / 8))), dim3(256), 0, s>>>((const uint16_t*)src, (uint16_t*)(ws + q.at),
-                                                                           rows, c, q.ld);
+PadRows pad_of(const void* src, char* ws, const Padded& q, long long rows, int c) {
+  return PadRows{(const uint16_t*)src, q.on ? (uint16_t*)(ws + q.at) : nullptr, rows, c, q.ld};
+}
+int pad(const PadRows& a, const PadRows& b, hipStream_t s) {
+  if (!a.dst && !b.dst) return MI_OK;
+  const long long na = a.dst ? a.rows * (a.cp / 8) : 0, nb = b.dst ? b.rows * (b.cp / 8) : 0;
+  pad_rows_kernel<<<dim3(blocks_for(na > nb ? na : nb), b.dst ? 2 : 1), dim3(256), 0, s>>>(PadBoth{{a, b}});
   return launched("padded copy");
 }
 const uint16_t* placed(const void* src, char* ws, const Padded& q) {
@@ -292,6 +336,8 @@ const uint16_t* placed(const void* src, char* ws, const Padded& q) {
 
 int check_sizes(int M, int N, int K, int act) {
   if (M < 0 || N < 0 || K < 0) return fail(MI_E_ARGS, "negative size M=%d N=%d K=%d", M, N, K);
+  constexpr int most = 0x7FFFFFFF - 1024;  // sizes are rounded up to blocks in 32 bits
+  if (M > most || N > most || K > most) return fail(MI_E_RANGE, "a size over %d (M=%d N=%d K=%d)", most, M, N, K);
   if (act < MI_ACT_NONE || act > MI_ACT_SILU) return fail(MI_E_ARGS, "unknown activation %d", act);
   const unsigned long long lim = kMaxOffset / 2;
   if ((unsigned long long)M * K > lim || (unsigned long long)K * N > lim || (unsigned long long)M * N > 1ull << 40)
@@ -364,6 +410,9 @@ int bwd_plan(const mi_epilogue_grad_args* a, char* ws, Bwd* b) {
     b->bytes += up256(b->dlhs.ws_bytes);
   }
   if (a->drhs) {
+    // The lhsT.rhs product's operands, and its loads past their ends.
+    const unsigned long long span = ((unsigned long long)M + 1024) * (unsigned long long)(b->kp > up8(a->N) ? b->kp : up8(a->N)) * 2ull;
+    if (span > kMaxOffset) return fail(MI_E_RANGE, "operand spans exceed 32-bit buffer offsets (%llu bytes)", span);
     b->drhs_padded = a->K % 8 != 0 || a->N % 8 != 0 || !at16(a->drhs);
     if (b->drhs_padded) {
       b->drhs_at = b->bytes;
@@ -437,16 +486,15 @@ int mi_matmul_epilogue_bf16(const mi_epilogue_args* a, const mi_tile_cfg* cfg, v
   o.N = N;
   o.act = a->activation;
   o.bias_f32 = a->bias_f32 != 0;
-  // (A block's rows of the outputs are within 32-bit offsets up to a million columns.)
-  o.vec = N % 8 == 0 && N <= 1 << 20 && at16(a->bias) && at16(a->residual) && at16(a->pre) && at16(a->out);
+  o.vec = N % 8 == 0 && N <= kWide && at16(a->bias) && at16(a->residual) && at16(a->pre) && at16(a->out);
   if (K == 0) {
     epi_sum_kernel<<<dim3(blocks_for((long long)M * (up8(N) / 8))), dim3(256), 0, s>>>(nullptr, 0, up8(N), o);
     return launched("epilogue of an empty product");
   }
   char* ws = (char*)workspace;
   const bool bt = a->rhs_transposed != 0;
-  if ((rc = pad(a->lhs, ws, f.lhs, M, K, s)) != MI_OK) return rc;
-  if ((rc = pad(a->rhs, ws, f.rhs, bt ? N : K, bt ? K : N, s)) != MI_OK) return rc;
+  rc = pad(pad_of(a->lhs, ws, f.lhs, M, K), pad_of(a->rhs, ws, f.rhs, bt ? N : K, bt ? K : N), s);
+  if (rc != MI_OK) return rc;
   return run(f.mm, o, (float*)(ws + f.part_at), s);
 }
 
@@ -496,12 +544,13 @@ int mi_matmul_epilogue_backward_bf16(const mi_epilogue_grad_args* a, void* works
   const int np = up8(N);
   if (a->dbias || b.dpre) {
     ActGrad g = {dout, act ? (const uint16_t*)a->pre : nullptr, b.dpre ? (uint16_t*)dpre : nullptr,
-                 a->dbias ? (float*)(ws + b.bias_at) : nullptr, M, N, np, a->activation,
-                 N % 8 == 0 && at16(a->dout) && at16(a->pre)};
+                 a->dbias ? (float*)(ws + b.bias_at) : nullptr, M, N, np, a->activation};
     const int xb = (np + 511) / 512, rows4 = (M + 3) / 4;
     int chunks = a->dbias ? b.chunks : 4096 / xb;
     chunks = chunks < 1 ? 1 : chunks > rows4 ? rows4 : chunks;
-    act_grad_kernel<<<dim3((unsigned)xb, (unsigned)chunks), dim3(256), 0, s>>>(g);
+    const dim3 grid((unsigned)xb, (unsigned)chunks);
+    if (N < 8) act_grad_kernel<1><<<grid, dim3(256), 0, s>>>(g);
+    else act_grad_kernel<8><<<grid, dim3(256), 0, s>>>(g);
     if ((rc = launched("activation gradient")) != MI_OK) return rc;
     if (a->dbias) {
       const mi::ColumnSum c = {g.part, {a->dbias, nullptr}, chunks, N};
@@ -512,18 +561,20 @@ int mi_matmul_epilogue_backward_bf16(const mi_epilogue_grad_args* a, void* works
     }
   }
   if (K == 0) return MI_OK;
-  if (!b.dpre && (a->dlhs || a->drhs) && (rc = pad(a->dout, ws, b.dout, M, N, s)) != MI_OK) return rc;
+  const PadRows none = {nullptr, nullptr, 0, 0, 0};
+  if (!b.dpre && (a->dlhs || a->drhs) && (rc = pad(pad_of(a->dout, ws, b.dout, M, N), none, s)) != MI_OK) return rc;
+  rc = pad(a->drhs ? pad_of(a->lhs, ws, b.lhs, M, K) : none,
+           a->dlhs ? pad_of(a->rhs, ws, b.rhs, bt ? N : K, bt ? K : N) : none, s);
+  if (rc != MI_OK) return rc;
   if (a->dlhs) {
-    if ((rc = pad(a->rhs, ws, b.rhs, bt ? N : K, bt ? K : N, s)) != MI_OK) return rc;
     EpiOut o = {};
     o.out = (uint16_t*)a->dlhs;
     o.M = M;
     o.N = K;
-    o.vec = K % 8 == 0 && K <= 1 << 20 && at16(a->dlhs);
+    o.vec = K % 8 == 0 && K <= kWide && at16(a->dlhs);
     if ((rc = run(b.dlhs, o, (float*)(ws + b.part_at), s)) != MI_OK) return rc;
   }
   if (a->drhs) {
-    if ((rc = pad(a->lhs, ws, b.lhs, M, K, s)) != MI_OK) return rc;
     const uint16_t* lhs = placed(a->lhs, ws, b.lhs);
     uint16_t* out = (uint16_t*)(b.drhs_padded ? (void*)(ws + b.drhs_at) : a->drhs);
     // drhs[K,N] = lhs^T . dpre, or drhs[N,K] = dpre^T . lhs: rows M contracted.
@@ -533,7 +584,7 @@ int mi_matmul_epilogue_backward_bf16(const mi_epilogue_grad_args* a, void* works
     if (b.drhs_padded) {
       const long long rows = bt ? N : K;
       const int c = bt ? K : N;
-      unpad_rows_kernel<<<dim3(blocks_for(rows * c)), dim3(256), 0, s>>>(out, (uint16_t*)a->drhs, rows, c, up8(c));
+      unpad_rows_kernel<<<dim3(blocks_for(rows * (up8(c) / 8))), dim3(256), 0, s>>>(out, (uint16_t*)a->drhs, rows, c, up8(c));
       return launched("gradient's copy");
     }
   }

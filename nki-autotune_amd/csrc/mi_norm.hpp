@@ -56,27 +56,46 @@ __device__ __forceinline__ Bf16 from_f32<Bf16>(float x) { return Bf16{__builtin_
 template <>
 __device__ __forceinline__ Fp16 from_f32<Fp16>(float x) { return Fp16{__builtin_bit_cast(uint16_t, (_Float16)x)}; }
 
-// 16 bytes of consecutive values at any address.
-template <class T>
+// W consecutive values (16 bytes of them) at any address.
+template <class T, int W = 16 / sizeof(T)>
 struct __attribute__((packed, aligned(sizeof(T)))) Pack {
-  static constexpr int V = 16 / sizeof(T);
+  static constexpr int V = W;
   T v[V];
 };
-template <class T>
-__device__ __forceinline__ Pack<T> load_pack(const T* p) {
-  return *(const Pack<T>*)p;
+template <class T, int W = 16 / sizeof(T)>
+__device__ __forceinline__ Pack<T, W> load_pack(const T* p) {
+  return *(const Pack<T, W>*)p;
 }
-template <class T>
-__device__ __forceinline__ void store_pack(T* p, const float (&in)[Pack<T>::V]) {
-  Pack<T> x;
+template <class T, int W>
+__device__ __forceinline__ void store_pack(T* p, const float (&in)[W]) {
+  Pack<T, W> x;
 #pragma unroll
-  for (int i = 0; i < Pack<T>::V; ++i) x.v[i] = from_f32<T>(in[i]);
-  *(Pack<T>*)p = x;
+  for (int i = 0; i < W; ++i) x.v[i] = from_f32<T>(in[i]);
+  *(Pack<T, W>*)p = x;
 }
-// A row of parameters: T, or fp32 where `f32`; `other` where there is none.
-template <class T>
-__device__ __forceinline__ float param_at(const void* p, bool f32, size_t at, float other) {
-  return !p ? other : f32 ? ((const float*)p)[at] : to_f32(((const T*)p)[at]);
+// Packs of a row of parameters, T or (`f32`) fp32; `other` where there is none.
+template <class T, int G, int W>
+__device__ __forceinline__ void load_params(const void* p, bool f32, const int (&at)[G], float other, float (&out)[G][W]) {
+  if (!p) {
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int i = 0; i < W; ++i) out[g][i] = other;
+  } else if (f32) {
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const Pack<float, W> x = load_pack<float, W>((const float*)p + at[g]);
+#pragma unroll
+      for (int i = 0; i < W; ++i) out[g][i] = x.v[i];
+    }
+  } else {
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const Pack<T, W> x = load_pack<T, W>((const T*)p + at[g]);
+#pragma unroll
+      for (int i = 0; i < W; ++i) out[g][i] = to_f32(x.v[i]);
+    }
+  }
 }
 
 // Sums a and b over the L lanes of a row: every lane gets both.  `turn`
@@ -130,6 +149,12 @@ struct RowSplit {
   __device__ __forceinline__ float mine(int g, int i, float x) const { return EXACT || i >= own[g] ? x : 0.0f; }
 };
 
+template <int V>
+__device__ __forceinline__ void fill(float (&x)[V], float to) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) x[i] = to;
+}
+
 struct LnFwd {
   const void *x, *weight, *bias;  // weight, bias: NULL for 1 and 0
   void* y;
@@ -141,7 +166,9 @@ struct LnFwd {
 };
 
 // GROUPS rows at a time in a block of GROUPS * L threads.  EXACT: D = E * L.
-template <class T, int E, int L, int GROUPS, bool EXACT>
+// KEEP: the parameters and the next row stay in registers (E = 32 of 1024
+// threads leaves no room for them).
+template <class T, int E, int L, int GROUPS, bool EXACT, bool KEEP>
 __global__ __launch_bounds__(L* GROUPS) void layer_norm_kernel(const LnFwd p) {
   constexpr int V = Pack<T>::V, G = E / V;
   static_assert(L <= 64 || GROUPS == 1, "rows of several waves have their block to themselves");
@@ -160,23 +187,21 @@ __global__ __launch_bounds__(L* GROUPS) void layer_norm_kernel(const LnFwd p) {
 #pragma unroll
     for (int g = 0; g < G; ++g) next[g] = load_pack(x + split.at[g]);
   };
-  fetch(row_of(r));
-  float w[G][V], b[G][V];
-#pragma unroll
-  for (int g = 0; g < G; ++g)
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      w[g][i] = param_at<T>(p.weight, p.params_f32, split.at[g] + i, 1.0f);
-      b[g][i] = param_at<T>(p.bias, p.params_f32, split.at[g] + i, 0.0f);
-    }
+  float w[KEEP ? G : 1][V], b[KEEP ? G : 1][V];
+  if constexpr (KEEP) {
+    fetch(row_of(r));
+    load_params<T>(p.weight, p.params_f32, split.at, 1.0f, w);
+    load_params<T>(p.bias, p.params_f32, split.at, 0.0f, b);
+  }
   int turn = 0;
   for (long long first = (long long)blockIdx.x * GROUPS; first < p.rows; first += step, r += step) {
     float v[G][V];
+    if constexpr (!KEEP) fetch(row_of(r));
 #pragma unroll
     for (int g = 0; g < G; ++g)
 #pragma unroll
       for (int i = 0; i < V; ++i) v[g][i] = to_f32(next[g].v[i]);
-    fetch(row_of(r + step));
+    if constexpr (KEEP) fetch(row_of(r + step));
     float sum = 0.0f, none = 0.0f;
 #pragma unroll
     for (int g = 0; g < G; ++g)
@@ -204,9 +229,18 @@ __global__ __launch_bounds__(L* GROUPS) void layer_norm_kernel(const LnFwd p) {
     T* y = (T*)p.y + (size_t)row_of(r) * (size_t)p.D;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
+      constexpr int K = KEEP ? 1 : 0;
+      if constexpr (!KEEP) {
+        // (Read again for each row, not once and then spilled.)
+        const void *weight = p.weight, *bias = p.bias;
+        asm volatile("" : "+s"(weight), "+s"(bias));
+        const int at[1] = {split.at[g]};
+        load_params<T>(weight, p.params_f32, at, 1.0f, w);
+        load_params<T>(bias, p.params_f32, at, 0.0f, b);
+      }
       float o[V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) o[i] = (v[g][i] - rest) * rstd * w[g][i] + b[g][i];
+      for (int i = 0; i < V; ++i) o[i] = (v[g][i] - rest) * rstd * w[K * g][i] + b[K * g][i];
       store_pack(y + split.at[g], o);
     }
     if (in_row == 0 && r < p.rows) {
@@ -216,9 +250,17 @@ __global__ __launch_bounds__(L* GROUPS) void layer_norm_kernel(const LnFwd p) {
   }
 }
 
-// Rows longer than registers hold, or shorter than 16 bytes: a block of B
-// threads per row reads it three times (from L2 after the first).
-template <class T, int B>
+// Rows longer than registers hold (W = 16 bytes), or shorter than 16 bytes (W
+// = 1): a block of B threads per row reads it three times (from L2 after the
+// first).  f(at, own) for each of a thread's packs.
+template <int B, int W, class F>
+__device__ __forceinline__ void each_pack(int tid, int D, F&& f) {
+  for (int d = tid * W; d < D; d += B * W) {
+    const int at = d + W <= D ? d : D - W;
+    f(at, d - at);
+  }
+}
+template <class T, int B, int W>
 __global__ __launch_bounds__(B) void layer_norm_long_kernel(const LnFwd p) {
   __shared__ float xs[2][B / 64][2];
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -227,21 +269,36 @@ __global__ __launch_bounds__(B) void layer_norm_long_kernel(const LnFwd p) {
   for (long long r = blockIdx.x; r < p.rows; r += gridDim.x) {
     const T* x = (const T*)p.x + (size_t)r * (size_t)p.ldx;
     float sum = 0.0f, none = 0.0f;
-    for (int d = tid; d < p.D; d += B) sum += to_f32(x[d]);
+    each_pack<B, W>(tid, p.D, [&](int at, int own) __attribute__((always_inline)) {
+      const Pack<T, W> v = load_pack<T, W>(x + at);
+#pragma unroll
+      for (int i = 0; i < W; ++i) sum += i >= own ? to_f32(v.v[i]) : 0.0f;
+    });
     row_sum2<B>(sum, none, xs, wave, lane, turn);
     float mean = sum * inv_d, rest = 0.0f, sq = 0.0f;
-    for (int d = tid; d < p.D; d += B) {
-      const float c = to_f32(x[d]) - mean;
-      rest += c;
-      sq += c * (c * inv_d);
-    }
+    each_pack<B, W>(tid, p.D, [&](int at, int own) __attribute__((always_inline)) {
+      const Pack<T, W> v = load_pack<T, W>(x + at);
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        const float c = i >= own ? to_f32(v.v[i]) - mean : 0.0f;
+        rest += c;
+        sq += c * (c * inv_d);
+      }
+    });
     row_sum2<B>(rest, sq, xs, wave, lane, turn);
     rest *= inv_d;
     const float rstd = norm_rstd(sq - rest * rest, p.eps);
     T* y = (T*)p.y + (size_t)r * (size_t)p.D;
-    for (int d = tid; d < p.D; d += B)
-      y[d] = from_f32<T>((to_f32(x[d]) - mean - rest) * rstd * param_at<T>(p.weight, p.params_f32, d, 1.0f) +
-                         param_at<T>(p.bias, p.params_f32, d, 0.0f));
+    each_pack<B, W>(tid, p.D, [&](int at, int) __attribute__((always_inline)) {
+      const Pack<T, W> v = load_pack<T, W>(x + at);
+      float w[1][W], b[1][W], o[W];
+      const int where[1] = {at};
+      load_params<T>(p.weight, p.params_f32, where, 1.0f, w);
+      load_params<T>(p.bias, p.params_f32, where, 0.0f, b);
+#pragma unroll
+      for (int i = 0; i < W; ++i) o[i] = (to_f32(v.v[i]) - mean - rest) * rstd * w[0][i] + b[0][i];
+      store_pack(y + at, o);
+    });
     if (tid == 0) {
       if (p.mean) p.mean[r] = mean + rest;
       if (p.rstd) p.rstd[r] = rstd;
@@ -259,7 +316,7 @@ struct LnBwd {
   bool weight_f32;
 };
 
-// GROUPS rows at a time in a block of GROUPS * L threads.  EXACT: D = E * L.
+// GROUPS rows at a time in a block of GROUPS * L threads; EXACT: as above.
 template <class T, int E, int L, int GROUPS, bool EXACT>
 __global__ __launch_bounds__(L* GROUPS) void layer_norm_bwd_kernel(const LnBwd p) {
   constexpr int V = Pack<T>::V, G = E / V, WPR = L < 64 ? 1 : L / 64;
@@ -286,16 +343,14 @@ __global__ __launch_bounds__(L* GROUPS) void layer_norm_bwd_kernel(const LnBwd p
     nmean = p.mean[at];
     nrstd = p.rstd[at];
   };
-  fetch(row_of(r));
   float w[G][V], dw[G][V], db[G][V];
+  fetch(row_of(r));
+  load_params<T>(p.weight, p.weight_f32, split.at, 1.0f, w);
 #pragma unroll
-  for (int g = 0; g < G; ++g)
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      w[g][i] = param_at<T>(p.weight, p.weight_f32, split.at[g] + i, 1.0f);
-      dw[g][i] = 0.0f;
-      db[g][i] = 0.0f;
-    }
+  for (int g = 0; g < G; ++g) {
+    fill(dw[g], 0.0f);
+    fill(db[g], 0.0f);
+  }
   int turn = 0;
   for (long long first = (long long)blockIdx.x * GROUPS; first < p.rows; first += step, r += step) {
     Pack<T> xv[G], dv[G];
@@ -309,7 +364,7 @@ __global__ __launch_bounds__(L* GROUPS) void layer_norm_bwd_kernel(const LnBwd p
     const bool live = r < p.rows;
     float sg = 0.0f, sgx = 0.0f;
 #pragma unroll
-    for (int g = 0; g < G; ++g)
+    for (int g = 0; g < G; ++g) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const float dy = to_f32(dv[g].v[i]), xh = (to_f32(xv[g].v[i]) - mean) * rstd;
@@ -320,6 +375,7 @@ __global__ __launch_bounds__(L* GROUPS) void layer_norm_bwd_kernel(const LnBwd p
         sg += gw;
         sgx += split.mine(g, i, gw * xh);
       }
+    }
     if (!p.dx) continue;
     row_sum2<L>(sg, sgx, xs[group], wave, lane, turn);
     sg *= inv_d;
@@ -341,12 +397,10 @@ __global__ __launch_bounds__(L* GROUPS) void layer_norm_bwd_kernel(const LnBwd p
   float* part_b = part_w + (size_t)gridDim.x * (size_t)p.D;
   if constexpr (GROUPS == 1) {
 #pragma unroll
-    for (int g = 0; g < G; ++g)
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        part_w[split.at[g] + i] = dw[g][i];
-        part_b[split.at[g] + i] = db[g][i];
-      }
+    for (int g = 0; g < G; ++g) {
+      store_pack(part_w + split.at[g], dw[g]);
+      store_pack(part_b + split.at[g], db[g]);
+    }
   } else {
     // The groups' sums in their order, one pack of columns at a time.
 #pragma unroll
@@ -371,7 +425,7 @@ __global__ __launch_bounds__(L* GROUPS) void layer_norm_bwd_kernel(const LnBwd p
 
 // Rows longer than registers hold, or shorter than 16 bytes: dx by a block of
 // B threads per row, and the column sums by layer_norm_columns_kernel.
-template <class T, int B>
+template <class T, int B, int W>
 __global__ __launch_bounds__(B) void layer_norm_bwd_long_kernel(const LnBwd p) {
   __shared__ float xs[2][B / 64][2];
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -381,38 +435,68 @@ __global__ __launch_bounds__(B) void layer_norm_bwd_long_kernel(const LnBwd p) {
     const T* x = (const T*)p.x + (size_t)r * (size_t)p.ldx;
     const T* dout = (const T*)p.dout + (size_t)r * (size_t)p.lddout;
     const float mean = p.mean[r], rstd = p.rstd[r];
+    // f(at, own, g, xh): a pack's dout * weight and normalised values.
+    const auto each = [&](auto&& f) __attribute__((always_inline)) {
+      each_pack<B, W>(tid, p.D, [&](int at, int own) __attribute__((always_inline)) {
+        const Pack<T, W> v = load_pack<T, W>(x + at), d = load_pack<T, W>(dout + at);
+        float w[1][W], g[W], xh[W];
+        const int where[1] = {at};
+        load_params<T>(p.weight, p.weight_f32, where, 1.0f, w);
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          g[i] = to_f32(d.v[i]) * w[0][i];
+          xh[i] = (to_f32(v.v[i]) - mean) * rstd;
+        }
+        f(at, own, g, xh);
+      });
+    };
     float sg = 0.0f, sgx = 0.0f;
-    for (int d = tid; d < p.D; d += B) {
-      const float g = to_f32(dout[d]) * param_at<T>(p.weight, p.weight_f32, d, 1.0f);
-      sg += g;
-      sgx += g * ((to_f32(x[d]) - mean) * rstd);
-    }
+    each([&](int, int own, const float(&g)[W], const float(&xh)[W]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        sg += i >= own ? g[i] : 0.0f;
+        sgx += i >= own ? g[i] * xh[i] : 0.0f;
+      }
+    });
     row_sum2<B>(sg, sgx, xs, wave, lane, turn);
     sg *= inv_d;
     sgx *= inv_d;
     T* dx = (T*)p.dx + (size_t)r * (size_t)p.D;
-    for (int d = tid; d < p.D; d += B) {
-      const float xh = (to_f32(x[d]) - mean) * rstd;
-      dx[d] = from_f32<T>(rstd * (to_f32(dout[d]) * param_at<T>(p.weight, p.weight_f32, d, 1.0f) - sg - xh * sgx));
-    }
+    each([&](int at, int, const float(&g)[W], const float(&xh)[W]) __attribute__((always_inline)) {
+      float o[W];
+#pragma unroll
+      for (int i = 0; i < W; ++i) o[i] = rstd * (g[i] - sg - xh[i] * sgx);
+      store_pack(dx + at, o);
+    });
   }
 }
 
-// Column sums over the rows of one chunk: blockIdx.x takes 256 columns,
-// blockIdx.y (of gridDim.y) every gridDim.y-th row.  part: [2][gridDim.y][D].
-template <class T>
+// Column sums over the rows of one chunk: blockIdx.x takes 256 packs of
+// columns, blockIdx.y (of gridDim.y) every gridDim.y-th row.  part:
+// [2][gridDim.y][D].
+template <class T, int W>
 __global__ __launch_bounds__(256) void layer_norm_columns_kernel(const LnBwd p) {
-  const int d = (int)blockIdx.x * 256 + (int)threadIdx.x;
+  const int d = ((int)blockIdx.x * 256 + (int)threadIdx.x) * W;
   if (d >= p.D) return;
-  float dw = 0.0f, db = 0.0f;
+  const int at = d + W <= p.D ? d : p.D - W;
+  float dw[W], db[W];
+  fill(dw, 0.0f);
+  fill(db, 0.0f);
+#pragma unroll 4
   for (long long r = blockIdx.y; r < p.rows; r += gridDim.y) {
-    const float dy = to_f32(((const T*)p.dout)[(size_t)r * (size_t)p.lddout + d]);
-    dw += dy * ((to_f32(((const T*)p.x)[(size_t)r * (size_t)p.ldx + d]) - p.mean[r]) * p.rstd[r]);
-    db += dy;
+    const Pack<T, W> v = load_pack<T, W>((const T*)p.x + (size_t)r * (size_t)p.ldx + at);
+    const Pack<T, W> g = load_pack<T, W>((const T*)p.dout + (size_t)r * (size_t)p.lddout + at);
+    const float mean = p.mean[r], rstd = p.rstd[r];
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const float dy = to_f32(g.v[i]);
+      dw[i] += dy * ((to_f32(v.v[i]) - mean) * rstd);
+      db[i] += dy;
+    }
   }
-  float* part_w = p.part + (size_t)blockIdx.y * (size_t)p.D;
-  part_w[d] = dw;
-  part_w[(size_t)gridDim.y * (size_t)p.D + d] = db;
+  float* part_w = p.part + (size_t)blockIdx.y * (size_t)p.D + at;
+  store_pack(part_w, dw);
+  store_pack(part_w + (size_t)gridDim.y * (size_t)p.D, db);
 }
 
 // (A kernel rather than a memset: memset nodes of a captured graph have given

@@ -100,7 +100,7 @@ def test_ordinary_calls_are_taken(gpu):
     assert n.newton_schulz(t.half(), 5, 1.0, 1.0, 1.0, 1e-7, None) is None
 
 
-def test_a_library_error_is_raised_by_either(gpu, monkeypatch):
+def test_a_library_error_is_raised_by_either(gpu):
     import torch
 
     import kernel_library as kl
@@ -111,5 +111,5 @@ def test_a_library_error_is_raised_by_either(gpu, monkeypatch):
     out = torch.empty(1, 2**31 - 8, dtype=torch.bfloat16, device=gpu)
     kl.layer_norm(lhs)
     for _ in range(2):
-        with pytest.raises(kl.epilogue._lib.KernelLibraryError, match="32-bit"):
+        with pytest.raises(kl.epilogue._lib.KernelLibraryError, match="rc=5"):
             kl.matmul_epilogue(lhs, wide, out=out)
