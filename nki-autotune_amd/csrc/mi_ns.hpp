@@ -199,38 +199,60 @@ __device__ __forceinline__ void ns_main(const NsMM& p, const uint16_t* a, const 
 #pragma unroll
   for (int j = 0; j < TN; ++j) read_b(0, 0, j);
 
-  // hi.hi, with lo's fragments read in its first half; three quarters in,
-  // every wave has them, and the loads of tile t+STAGES go out into the stage,
-  // up to the end of hi.lo.  Then tile t+1 has landed, and its hi fragments are
-  // read over lo.hi, A's at once (nobody needs this tile's any more), B's
-  // column by column as this tile's are done with.
+  // hi.hi, with lo's fragments read in its first half, then hi.lo.  Then tile
+  // t+1 has landed, and its hi fragments are read over lo.hi, A's at once
+  // (nobody needs this tile's any more), B's column by column as this tile's
+  // are done with.
+  //
+  // The loads of tile t+STAGES go out once every wave has this tile's
+  // fragments.  Two stages (large blocks) have a barrier of their own for it
+  // three quarters into hi.hi, so the loads are in flight for the rest of it,
+  // hi.lo and lo.hi and the next tile's first two; more stages (small blocks)
+  // do with the one that tile t+1 needs (1024 x 1024: 182 -> 174 us).
+  //
+  // Small blocks are bound by what one unit draws from L2, about 100 GB/s (16
+  // KB a tile in 0.15 us): a second group of waves taking every other tile
+  // left 512 x 512 at 121 us (127 with it).
   constexpr int HM = NM / 2, QM = NM / 4, SLOTS = NM - HM - QM + NM;
+  constexpr bool EARLY = STAGES == 2;
   auto tile = [&](int t, auto cur_c) __attribute__((always_inline)) {
     constexpr int cur = decltype(cur_c)::value, nxt = (cur + 1) % STAGES;
+    const int t_new = clamp(t + STAGES);
 #pragma unroll
     for (int i = 0; i < TM; ++i) read_a(cur, 1, i);
 #pragma unroll
     for (int j = 0; j < TN; ++j) read_b(cur, 1, j);
-    mfmas(0, 0, 0, HM);
-    interleave_mfma_ds<HM, READS>();
-    mfmas(0, 0, HM, HM + QM);
-    __builtin_amdgcn_sched_barrier(0);
-    __syncthreads();
-    const int t_new = clamp(t + STAGES);
-    static_for<SLOTS>([&](auto x_c) __attribute__((always_inline)) {
-      constexpr int x = decltype(x_c)::value;
-#pragma unroll
-      for (int q = x * LPT / SLOTS; q < (x + 1) * LPT / SLOTS; ++q) issue_one(q, t_new, cur);
-      if constexpr (x < NM - HM - QM) mfmas(0, 0, HM + QM + x, HM + QM + x + 1);
-      else mfmas(0, 1, x - (NM - HM - QM), x - (NM - HM - QM) + 1);
+    if constexpr (EARLY) {
+      mfmas(0, 0, 0, HM);
+      interleave_mfma_ds<HM, READS>();
+      mfmas(0, 0, HM, HM + QM);
       __builtin_amdgcn_sched_barrier(0);
-    });
-    vm_wait<(STAGES - 1) * LPT>();
+      __syncthreads();
+      static_for<SLOTS>([&](auto x_c) __attribute__((always_inline)) {
+        constexpr int x = decltype(x_c)::value;
+#pragma unroll
+        for (int q = x * LPT / SLOTS; q < (x + 1) * LPT / SLOTS; ++q) issue_one(q, t_new, cur);
+        if constexpr (x < NM - HM - QM) mfmas(0, 0, HM + QM + x, HM + QM + x + 1);
+        else mfmas(0, 1, x - (NM - HM - QM), x - (NM - HM - QM) + 1);
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      vm_wait<LPT>();
+    } else {
+      mfmas(0, 0, 0, NM);
+      interleave_mfma_ds<NM, READS>();
+      mfmas(0, 1, 0, NM);
+      __builtin_amdgcn_sched_barrier(0);
+      vm_wait<(STAGES - 2) * LPT>();
+    }
     __syncthreads();
     static_for<TN>([&](auto j_c) __attribute__((always_inline)) {
       constexpr int j = decltype(j_c)::value;
 #pragma unroll
       for (int i = j * TM / TN; i < (j + 1) * TM / TN; ++i) read_a(nxt, 0, i);
+      if constexpr (!EARLY) {
+#pragma unroll
+        for (int q = j * LPT / TN; q < (j + 1) * LPT / TN; ++q) issue_one(q, t_new, cur);
+      }
       mfmas(1, 0, j * TM, (j + 1) * TM);
       read_b(nxt, 0, j);
       __builtin_amdgcn_sched_barrier(0);
