@@ -3,10 +3,12 @@
 // mi_mm_epi.hpp).
 #include "mi_capi_internal.hpp"
 #include "mi_epi_table.hpp"
+#include "mi_mm_any.hpp"
 #include "mi_norm.hpp"
 
 namespace {
 
+using mi::AnyMM;
 using mi::EpiEntry;
 using mi::EpiMM;
 using mi::EpiOut;
@@ -46,20 +48,28 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(const PadBoth both) {
   }
 }
 
-// dst[r][0, c) = src[r][0, c) of rows cp apart (dst rows c apart): the way back.
-__global__ __launch_bounds__(256) void unpad_rows_kernel(const uint16_t* __restrict__ src, uint16_t* __restrict__ dst,
-                                                         long long rows, int c, int cp) {
-  const int groups = cp / 8;
-  const long long n = rows * groups;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-    const long long r = i / groups;
-    const int d = (int)(i - r * groups) * 8;
-    const uint16_t* s = src + (size_t)r * (size_t)cp + d;
-    uint16_t* t = dst + (size_t)r * (size_t)c + d;
-    if (d + 8 <= c) {
-      *(mi::Pack<uint16_t>*)t = mi::load_pack(s);
-    } else {
-      for (int k = 0; d + k < c; ++k) t[k] = s[k];
+// dst[c][0, rp) = src[0, rows)[c], then zeros: an operand whose rows are
+// contracted, turned.  64 x 64 pieces through LDS.
+__global__ __launch_bounds__(256) void turn_rows_kernel(const uint16_t* __restrict__ src, uint16_t* __restrict__ dst,
+                                                        int rows, int cols, int ld, int rp) {
+  __shared__ uint16_t tile[64][66];
+  const int tid = (int)threadIdx.x, c0 = (int)blockIdx.x * 64;
+  for (int r0 = (int)blockIdx.y * 64; r0 < rp; r0 += (int)gridDim.y * 64) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int r = r0 + (tid >> 6) + 4 * i, c = c0 + (tid & 63);
+      tile[tid & 63][(tid >> 6) + 4 * i] = r < rows && c < cols ? src[(size_t)r * (size_t)ld + c] : (uint16_t)0;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int c = (tid >> 3) + 32 * i, r = (tid & 7) * 8;
+      if (c0 + c >= cols || r0 + r >= rp) continue;
+      mi::Pack<uint16_t> v;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v.v[k] = tile[c][r + k];
+      *(mi::Pack<uint16_t>*)(dst + (size_t)(c0 + c) * (size_t)rp + r0 + r) = v;
     }
   }
 }
@@ -258,13 +268,15 @@ mi_tile_cfg pick(int M, int N, int K, bool bt) {
   return best;
 }
 
-// One product A . B or A . B^T with an epilogue, operands already in rows of
-// 16 bytes.
+// One product A . B or A . B^T with an epilogue: of operands in rows of 16
+// bytes, or (any) as they are.
 struct Product {
   EpiMM mm;
   const EpiEntry* e;
   int ldw;
   size_t ws_bytes;
+  bool any, bt;
+  AnyMM as_is;
 };
 int plan(const uint16_t* a, int lda, const uint16_t* b, int ldb, long long b_rows, int M, int N, int K, bool bt,
          const mi_tile_cfg* cfg, Product* out) {
@@ -285,6 +297,7 @@ int plan(const uint16_t* a, int lda, const uint16_t* b, int ldb, long long b_row
                                        : ((unsigned long long)K + c.block_k) * ldb * 2ull + 2ull * c.block_n;
   if (a_span > kMaxOffset || b_span > kMaxOffset)
     return fail(MI_E_RANGE, "operand spans exceed 32-bit buffer offsets (%llu, %llu bytes)", a_span, b_span);
+  out->any = false;
   out->e = e;
   out->ldw = up8(N);
   out->ws_bytes = c.split_k > 1 ? (size_t)c.split_k * (size_t)M * (size_t)out->ldw * 4 : 0;
@@ -294,17 +307,54 @@ int plan(const uint16_t* a, int lda, const uint16_t* b, int ldb, long long b_row
                   c.group_m > 0 ? c.group_m : 8, c.split_k};
   return MI_OK;
 }
-int run(const Product& p, const EpiOut& o, float* ws, hipStream_t s) {
-  if (p.mm.parts > 1) {
-    p.e->split(p.mm, ws, p.ldw, s);
-    const int rc = launched("epilogue product");
-    if (rc != MI_OK) return rc;
-    epi_sum_kernel<<<dim3(blocks_for((long long)o.M * (p.ldw / 8))), dim3(256), 0, s>>>(ws, p.mm.parts, p.ldw, o);
-    return launched("sum of the parts");
-  }
-  p.e->direct(p.mm, o, s);
-  return launched("epilogue product");
+// The blocks of the products of operands as they are: 32 x 128, or 64 x 64
+// past 32 rows.
+int any_bm(int M) { return M <= 32 ? 32 : 64; }
+int any_bn(int M) { return M <= 32 ? 128 : 64; }
+template <int BM, int BN, bool BT>
+void any_launch(const AnyMM& p, const EpiOut& o, float* ws, int ldw, hipStream_t s) {
+  const unsigned tiles = (unsigned)((p.M + BM - 1) / BM) * (unsigned)((p.N + BN - 1) / BN);
+  if (p.parts > 1) mi::mm_any_split_kernel<BM, BN, BT><<<dim3(tiles * (unsigned)p.parts), dim3(256), 0, s>>>(p, ws, ldw);
+  else mi::mm_any_kernel<BM, BN, BT><<<dim3(tiles), dim3(256), 0, s>>>(p, o);
 }
+// A product of operands as they are: as many parts as fill the chip four
+// blocks a unit.
+void plan_any(const uint16_t* a, int lda, const uint16_t* b, int ldb, int M, int N, int K, bool bt, Product* out) {
+  const long long tiles = (long long)((M + any_bm(M) - 1) / any_bm(M)) * ((N + any_bn(M) - 1) / any_bn(M));
+  const int kt = (K + 63) / 64, cus = mi::capi::device_cus();
+  int parts = 1;
+  if (N <= kWide)
+    while (parts < 8 && tiles * parts * 2 <= 4ll * cus && kt / (parts * 2) >= 4) parts *= 2;
+  const int each = (kt + parts - 1) / parts;
+  parts = (kt + each - 1) / each;
+  out->any = true;
+  out->bt = bt;
+  out->as_is = AnyMM{a, b, M, N, K, lda, ldb, 8, parts};
+  out->ldw = up8(N);
+  out->ws_bytes = parts > 1 ? (size_t)parts * (size_t)M * (size_t)out->ldw * 4 : 0;
+}
+int run(const Product& p, const EpiOut& o, float* ws, hipStream_t s) {
+  const int parts = p.any ? p.as_is.parts : p.mm.parts;
+  if (p.any) {
+    if (p.as_is.M <= 32) p.bt ? any_launch<32, 128, true>(p.as_is, o, ws, p.ldw, s) : any_launch<32, 128, false>(p.as_is, o, ws, p.ldw, s);
+    else p.bt ? any_launch<64, 64, true>(p.as_is, o, ws, p.ldw, s) : any_launch<64, 64, false>(p.as_is, o, ws, p.ldw, s);
+  } else if (parts > 1) {
+    p.e->split(p.mm, ws, p.ldw, s);
+  } else {
+    p.e->direct(p.mm, o, s);
+  }
+  const int rc = launched("epilogue product");
+  if (rc != MI_OK || parts == 1) return rc;
+  epi_sum_kernel<<<dim3(blocks_for((long long)o.M * (p.ldw / 8))), dim3(256), 0, s>>>(ws, parts, p.ldw, o);
+  return launched("sum of the parts");
+}
+// Whether a product some of whose operands would need padded copies takes them
+// as they are instead.  A copy reads and writes its operand once more, which
+// for few rows is most of the work: 16 x 8001 x 12345 takes 39 us as it is and
+// 153 with copies (198 MB: 5 TB/s and 1.3), 200 x 4001 x 4001 37 and 38.  Past
+// that the padded kernels' larger blocks win: 500 x 2001 x 3001 31 and 25 us,
+// 1000 x 5001 x 4001 110 and 78.
+bool better_as_is(int M, int N, int K, bool bt) { return M <= 256 && K >= 8 && (bt || N >= 8); }
 
 // An operand that needs padded rows: its copy's place in the workspace.
 struct Padded {
@@ -360,6 +410,12 @@ int fwd_plan(const mi_epilogue_args* a, const mi_tile_cfg* cfg, char* ws, Fwd* f
   const int b_rows = bt ? a->N : a->K, b_cols = bt ? a->K : a->N;
   f->lhs = padded(a->lhs, a->M, a->K, &f->bytes);
   f->rhs = padded(a->rhs, b_rows, b_cols, &f->bytes);
+  if (f->bytes && !cfg && better_as_is(a->M, a->N, a->K, bt)) {
+    *f = Fwd{};
+    plan_any((const uint16_t*)a->lhs, a->K, (const uint16_t*)a->rhs, b_cols, a->M, a->N, a->K, bt, &f->mm);
+    f->bytes = f->mm.ws_bytes;
+    return MI_OK;
+  }
   f->part_at = f->bytes;
   const int prc = plan(placed(a->lhs, ws, f->lhs), f->lhs.ld, placed(a->rhs, ws, f->rhs), f->rhs.ld, b_rows, a->M, a->N,
                        f->lhs.ld, bt, cfg, &f->mm);
@@ -370,10 +426,10 @@ int fwd_plan(const mi_epilogue_args* a, const mi_tile_cfg* cfg, char* ws, Fwd* f
 struct Bwd {
   Padded dout, lhs, rhs;      // dout: dpre's place, or dout's padded copy
   bool dpre;                  // dout * act'(pre) goes to that place
-  Product dlhs;
-  size_t part_at, drhs_at, bias_at, bytes;
-  int chunks, kp;
-  bool drhs_padded;
+  Product dlhs, drhs;
+  bool turned;                // drhs by a product of its turned operand (else mi_matmul_lhsT_rhs_bf16)
+  size_t dlhs_part, drhs_part, turn_at, bias_at, bytes;
+  int chunks, rp;
 };
 int bwd_plan(const mi_epilogue_grad_args* a, char* ws, Bwd* b) {
   const int rc = check_sizes(a->M, a->N, a->K, a->activation);
@@ -382,41 +438,59 @@ int bwd_plan(const mi_epilogue_grad_args* a, char* ws, Bwd* b) {
   if (a->M == 0 || a->N == 0) return MI_OK;
   const bool bt = a->rhs_transposed != 0;
   const long long M = a->M;
-  b->kp = up8(a->K);
+  const int N = a->N, K = a->K;
+  const auto take = [&](size_t n) {
+    const size_t at = b->bytes;
+    b->bytes += up256(n);
+    return at;
+  };
   if (a->dbias) {
-    const int xb = (up8(a->N) + 511) / 512;
+    const int xb = (up8(N) + 511) / 512;
     const int rows4 = (a->M + 3) / 4, want = 2048 / xb;
     b->chunks = want < 1 ? 1 : want > 256 ? 256 : want;
     if (b->chunks > rows4) b->chunks = rows4;
-    b->bias_at = b->bytes;
-    b->bytes += up256((size_t)b->chunks * a->N * 4);
+    b->bias_at = take((size_t)b->chunks * N * 4);
   }
-  if (a->K == 0 || (!a->dlhs && !a->drhs)) return MI_OK;
+  if (K == 0 || (!a->dlhs && !a->drhs)) return MI_OK;
   b->dpre = a->activation != MI_ACT_NONE;
-  b->dout = Padded{b->dpre || a->N % 8 != 0 || !at16(a->dout), up8(a->N), 0, 0};
+  b->dout = Padded{b->dpre || N % 8 != 0 || !at16(a->dout), up8(N), 0, 0};
   if (b->dout.on) {
-    b->dout.at = b->bytes;
     b->dout.bytes = (size_t)M * b->dout.ld * 2;
-    b->bytes += up256(b->dout.bytes);
+    b->dout.at = take(b->dout.bytes);
   }
-  if (a->drhs) b->lhs = padded(a->lhs, M, a->K, &b->bytes);
+  const uint16_t* dpre = placed(a->dout, ws, b->dout);
   if (a->dlhs) {
-    b->rhs = padded(a->rhs, bt ? a->N : a->K, bt ? a->K : a->N, &b->bytes);
     // dlhs[M,K] = dpre[M,N] . rhs^T: rhs[K,N] is K-contiguous for it, rhs[N,K] is not.
-    const int prc = plan(placed(a->dout, ws, b->dout), b->dout.ld, placed(a->rhs, ws, b->rhs), b->rhs.ld,
-                         bt ? a->N : a->K, a->M, a->K, b->dout.ld, !bt, nullptr, &b->dlhs);
-    if (prc != MI_OK) return prc;
-    b->part_at = b->bytes;
-    b->bytes += up256(b->dlhs.ws_bytes);
+    const int rows = bt ? N : K, cols = bt ? K : N;
+    const bool copies = cols % 8 != 0 || !at16(a->rhs);
+    if (copies && better_as_is(a->M, K, N, !bt)) {
+      plan_any(dpre, b->dout.ld, (const uint16_t*)a->rhs, cols, a->M, K, N, !bt, &b->dlhs);
+    } else {
+      b->rhs = padded(a->rhs, rows, cols, &b->bytes);
+      const int prc = plan(dpre, b->dout.ld, placed(a->rhs, ws, b->rhs), b->rhs.ld, rows, a->M, K, b->dout.ld, !bt,
+                           nullptr, &b->dlhs);
+      if (prc != MI_OK) return prc;
+    }
+    b->dlhs_part = take(b->dlhs.ws_bytes);
   }
   if (a->drhs) {
-    // The lhsT.rhs product's operands, and its loads past their ends.
-    const unsigned long long span = ((unsigned long long)M + 1024) * (unsigned long long)(b->kp > up8(a->N) ? b->kp : up8(a->N)) * 2ull;
-    if (span > kMaxOffset) return fail(MI_E_RANGE, "operand spans exceed 32-bit buffer offsets (%llu bytes)", span);
-    b->drhs_padded = a->K % 8 != 0 || a->N % 8 != 0 || !at16(a->drhs);
-    if (b->drhs_padded) {
-      b->drhs_at = b->bytes;
-      b->bytes += up256((size_t)b->kp * up8(a->N) * 2);
+    // The lhsT.rhs product stores whole 16-byte pieces of rows.  Other results
+    // take the operand whose columns are the result's rows turned, and the
+    // epilogue product of it: drhs[K,N] = (lhs^T) . dpre, drhs[N,K] = (dpre^T) . lhs.
+    b->turned = K % 8 != 0 || N % 8 != 0 || !at16(a->drhs);
+    if (!b->turned || bt) b->lhs = padded(a->lhs, M, K, &b->bytes);
+    const uint16_t* lhs = placed(a->lhs, ws, b->lhs);
+    if (b->turned) {
+      b->rp = up8(a->M);
+      b->turn_at = take((size_t)(bt ? N : K) * b->rp * 2);
+      const int prc = plan((const uint16_t*)(ws + b->turn_at), b->rp, bt ? lhs : dpre, bt ? b->lhs.ld : b->dout.ld, M,
+                           bt ? N : K, bt ? K : N, b->rp, false, nullptr, &b->drhs);
+      if (prc != MI_OK) return prc;
+      b->drhs_part = take(b->drhs.ws_bytes);
+    } else {
+      // Its operands, and its loads past their ends.
+      const unsigned long long span = ((unsigned long long)M + 1024) * (unsigned long long)(K > N ? K : N) * 2ull;
+      if (span > kMaxOffset) return fail(MI_E_RANGE, "operand spans exceed 32-bit buffer offsets (%llu bytes)", span);
     }
   }
   return MI_OK;
@@ -563,30 +637,29 @@ int mi_matmul_epilogue_backward_bf16(const mi_epilogue_grad_args* a, void* works
   if (K == 0) return MI_OK;
   const PadRows none = {nullptr, nullptr, 0, 0, 0};
   if (!b.dpre && (a->dlhs || a->drhs) && (rc = pad(pad_of(a->dout, ws, b.dout, M, N), none, s)) != MI_OK) return rc;
-  rc = pad(a->drhs ? pad_of(a->lhs, ws, b.lhs, M, K) : none,
-           a->dlhs ? pad_of(a->rhs, ws, b.rhs, bt ? N : K, bt ? K : N) : none, s);
+  rc = pad(pad_of(a->lhs, ws, b.lhs, M, K), pad_of(a->rhs, ws, b.rhs, bt ? N : K, bt ? K : N), s);
   if (rc != MI_OK) return rc;
-  if (a->dlhs) {
+  const auto store_to = [](void* p, int rows, int cols) {
     EpiOut o = {};
-    o.out = (uint16_t*)a->dlhs;
-    o.M = M;
-    o.N = K;
-    o.vec = K % 8 == 0 && K <= kWide && at16(a->dlhs);
-    if ((rc = run(b.dlhs, o, (float*)(ws + b.part_at), s)) != MI_OK) return rc;
+    o.out = (uint16_t*)p;
+    o.M = rows;
+    o.N = cols;
+    o.vec = cols % 8 == 0 && cols <= kWide && at16(p);
+    return o;
+  };
+  if (a->dlhs && (rc = run(b.dlhs, store_to(a->dlhs, M, K), (float*)(ws + b.dlhs_part), s)) != MI_OK) return rc;
+  if (a->drhs && b.turned) {
+    const int cols = bt ? N : K;
+    turn_rows_kernel<<<dim3((unsigned)((cols + 63) / 64), (unsigned)((M + 63) / 64 < 4096 ? (M + 63) / 64 : 4096)), dim3(256), 0, s>>>(
+        bt ? dpre : (const uint16_t*)a->lhs, (uint16_t*)(ws + b.turn_at), M, cols, bt ? b.dout.ld : K, b.rp);
+    if ((rc = launched("turned operand")) != MI_OK) return rc;
+    return run(b.drhs, store_to(a->drhs, cols, bt ? K : N), (float*)(ws + b.drhs_part), s);
   }
   if (a->drhs) {
-    const uint16_t* lhs = placed(a->lhs, ws, b.lhs);
-    uint16_t* out = (uint16_t*)(b.drhs_padded ? (void*)(ws + b.drhs_at) : a->drhs);
     // drhs[K,N] = lhs^T . dpre, or drhs[N,K] = dpre^T . lhs: rows M contracted.
-    rc = bt ? mi::capi::matmul_lhsT_rhs_bf16(dpre, lhs, out, np, b.kp, M, nullptr, stream, nullptr, 0)
-            : mi::capi::matmul_lhsT_rhs_bf16(lhs, dpre, out, b.kp, np, M, nullptr, stream, nullptr, 0);
-    if (rc != MI_OK) return rc;
-    if (b.drhs_padded) {
-      const long long rows = bt ? N : K;
-      const int c = bt ? K : N;
-      unpad_rows_kernel<<<dim3(blocks_for(rows * (up8(c) / 8))), dim3(256), 0, s>>>(out, (uint16_t*)a->drhs, rows, c, up8(c));
-      return launched("gradient's copy");
-    }
+    const uint16_t* lhs = placed(a->lhs, ws, b.lhs);
+    return bt ? mi::capi::matmul_lhsT_rhs_bf16(dpre, lhs, a->drhs, N, K, M, nullptr, stream, nullptr, 0)
+              : mi::capi::matmul_lhsT_rhs_bf16(lhs, dpre, a->drhs, K, N, M, nullptr, stream, nullptr, 0);
   }
   return MI_OK;
 }

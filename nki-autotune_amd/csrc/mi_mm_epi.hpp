@@ -410,7 +410,7 @@ __device__ __forceinline__ void unpack8(u32x4_t w, float (&v)[8]) {
 }
 
 // pre = v + bias; out = act(pre) + residual.  `vec`: N is a multiple of 8 and
-// every pointer 16-byte aligned; otherwise elements go one by one.
+// every pointer 16-byte aligned (EpiVec); otherwise as here.
 struct EpiOut {
   const void* bias;
   const uint16_t* residual;
@@ -426,24 +426,7 @@ struct EpiOut {
   }
   __device__ __forceinline__ void columns(int n) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) b[i] = 0.0f;
-    if (!bias) return;
-    if (vec && n < N) {
-      if (bias_f32) {
-        const f32x4_t lo = *(const f32x4_t*)((const float*)bias + n), hi = *(const f32x4_t*)((const float*)bias + n + 4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          b[i] = lo[i];
-          b[4 + i] = hi[i];
-        }
-      } else {
-        unpack8(*(const u32x4_t*)((const uint16_t*)bias + n), b);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (n + i < N) b[i] = bias_at(n + i);
-    }
+    for (int i = 0; i < 8; ++i) b[i] = bias && n + i < N ? bias_at(n + i) : 0.0f;
   }
   __device__ __forceinline__ void fetch(int, int, int) {}
   __device__ __forceinline__ void arrived() {}
@@ -451,36 +434,39 @@ struct EpiOut {
     const int m = m0 + r;
     if (m >= M || n >= N) return;
     const size_t at = (size_t)m * (size_t)N + n;
+    const bool whole = n + 8 <= N;
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] += b[i];
-    if (pre) {
-      if (vec) {
-        *(u32x4_t*)(pre + at) = pack8(v);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (n + i < N) pre[at + i] = (uint16_t)pack_bf16x2(v[i], 0.0f);
-      }
-    }
+    if (pre) put(pre + at, n, whole, v);
     with_act(act, [&](auto a_c) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = act_value<decltype(a_c)::value>(v[i]);
     });
-    if (vec) {
-      if (residual) {
+    if (residual) {
+      if (whole) {
         float x[8];
-        unpack8(*(const u32x4_t*)(residual + at), x);
+        unpack8(((const Piece*)(residual + at))->v, x);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] += x[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (n + i < N) v[i] += bf16lo((uint32_t)residual[at + i]);
       }
-      *(u32x4_t*)(out + at) = pack8(v);
+    }
+    put(out + at, n, whole, v);
+  }
+  // 16 bytes at any address.
+  struct __attribute__((packed, aligned(2))) Piece {
+    u32x4_t v;
+  };
+  __device__ __forceinline__ void put(uint16_t* p, int n, bool whole, const float (&v)[8]) const {
+    if (whole) {
+      ((Piece*)p)->v = pack8(v);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (n + i < N) {
-          if (residual) v[i] += bf16lo((uint32_t)residual[at + i]);
-          out[at + i] = (uint16_t)pack_bf16x2(v[i], 0.0f);
-        }
+        if (n + i < N) p[i] = (uint16_t)pack_bf16x2(v[i], 0.0f);
     }
   }
 };

@@ -48,6 +48,35 @@ def test_shapes(gpu, M, N, K, transposed):
     _check(lhs, rhs, None, "none", None, transposed, kl.matmul_epilogue(lhs, rhs, rhs_transposed=transposed))
 
 
+@pytest.mark.parametrize("transposed", [False, True])
+@pytest.mark.parametrize("M,N,K", [(1, 8, 8), (1, 9, 1000), (2, 4097, 71), (31, 129, 65), (32, 128, 127), (33, 8, 9),
+                                   (40, 1001, 2049), (64, 65, 4099), (100, 200, 201), (256, 300, 333), (257, 300, 333),
+                                   (600, 77, 90), (5, 7, 100), (5, 100, 7)])
+def test_odd_sizes_as_they_are_and_copied(gpu, M, N, K, transposed):
+    """Rows that do not start on 16 bytes: few of them go through registers (whole and partial pieces, tiles and parts),
+    more are copied to padded ones; aligned sizes at odd addresses too, and infinities that must not leave the last
+    piece."""
+    import torch
+
+    import kernel_library as kl
+
+    print(f"matmul_epilogue {M}x{N}x{K} {transposed}", flush=True)
+    for off in (0, 1, 3):
+        lhs, rhs, b, r = _inputs(M, N, K, gpu, transposed, "float32")
+
+        def at(t):
+            big = torch.full((t.numel() + 64,), float("inf"), dtype=t.dtype, device=gpu)
+            view = big[16 + off:16 + off + t.numel()].view(t.shape)
+            view.copy_(t)
+            return view
+
+        out = kl.matmul_epilogue(at(lhs), at(rhs), b, "silu", at(r), rhs_transposed=transposed)
+        _check(lhs, rhs, b, "silu", r, transposed, out)
+        pre = r
+        got = kl.matmul_epilogue_backward(at(r), at(lhs), at(rhs), "silu", at(pre), b, rhs_transposed=transposed)
+        _check_backward(r, lhs, rhs, "silu", pre, transposed, *got)
+
+
 @pytest.mark.parametrize("act", ACTIVATIONS)
 @pytest.mark.parametrize("bias,residual", [("", False), ("bfloat16", False), ("float32", True), ("", True)])
 def test_epilogues(gpu, act, bias, residual):

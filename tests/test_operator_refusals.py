@@ -127,7 +127,7 @@ BIG = 2**31 - 1
     (dict(out=_at(0) + 64 * 64 * 2 - 2), _lib.MI_E_ARGS),
     (dict(pre=_at(4)), _lib.MI_E_ARGS),
     (dict(pre=_at(2)), _lib.MI_E_ARGS),
-    (dict(out=_at(9), K=63), _lib.MI_E_ARGS),  # the workspace
+    (dict(out=_at(9), M=512, K=63), _lib.MI_E_ARGS),  # the workspace
     (dict(M=0, lhs=None, out=None), _lib.MI_OK),
     (dict(N=0, rhs=None, out=None), _lib.MI_OK),
 ])
@@ -161,12 +161,19 @@ def test_matmul_epilogue_wide_outputs_are_not_split():
 
 def test_matmul_epilogue_workspace():
     L, need = _lib.lib(), ctypes.c_ulonglong()
-    for kw, copies in ((dict(), 0), (dict(K=63), 1), (dict(K=63, rhs_transposed=1), 2), (dict(N=63), 1),
-                       (dict(N=63, rhs_transposed=1), 0), (dict(lhs=_at(0) + 2), 1), (dict(rhs=_at(1) + 8), 1), (dict(K=0), 0), (dict(M=0), 0)):
-        assert _code(L.mi_matmul_epilogue_workspace, _mm(**kw), None, ctypes.byref(need)) == 0
-        assert need.value == copies * 64 * 64 * 2, kw
-    assert _code(L.mi_matmul_epilogue_bf16, _mm(K=63), None, None, 0, None) == _lib.MI_E_ARGS
-    assert _code(L.mi_matmul_epilogue_bf16, _mm(K=63), None, _at(9) + 2, GIB, None) == _lib.MI_E_ARGS
+    for kw, copies in ((dict(), 0), (dict(K=63), 512), (dict(K=63, rhs_transposed=1), 512 + 64), (dict(N=63), 64),
+                       (dict(N=63, rhs_transposed=1), 0), (dict(lhs=_at(0) + 2), 512), (dict(rhs=_at(1) + 8), 64),
+                       (dict(K=0), 0), (dict(M=0), 0)):
+        assert _code(L.mi_matmul_epilogue_workspace, _mm(**(dict(M=512) | kw)), None, ctypes.byref(need)) == 0
+        assert need.value == copies * 64 * 2, kw
+    assert _code(L.mi_matmul_epilogue_bf16, _mm(M=512, K=63), None, None, 0, None) == _lib.MI_E_ARGS
+    assert _code(L.mi_matmul_epilogue_bf16, _mm(M=512, K=63), None, _at(9) + 2, GIB, None) == _lib.MI_E_ARGS
+    # Few rows: no copies, unless a config asks for the kernels that need them or there is no whole 16-byte piece.
+    c = kl.TileConfig(64, 64, 64, 4, 2).to_c()
+    for kw, cfg, copies in ((dict(K=63), None, 0), (dict(N=63), None, 0), (dict(K=63), ctypes.byref(c), 64),
+                            (dict(K=7), None, 8), (dict(N=7), None, 8)):
+        assert _code(L.mi_matmul_epilogue_workspace, _mm(**kw), cfg, ctypes.byref(need)) == 0
+        assert need.value == copies * 64 * 2, kw
     assert L.mi_matmul_epilogue_workspace(None, None, ctypes.byref(need)) == _lib.MI_E_ARGS
     assert L.mi_matmul_epilogue_bf16(None, None, None, 0, None) == _lib.MI_E_ARGS
 
