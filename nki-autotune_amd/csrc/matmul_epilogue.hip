@@ -48,6 +48,24 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(const PadBoth both) {
   }
 }
 
+// dst[r][0, c) = src[r][0, c) of rows cp apart (dst rows c apart): the way back.
+__global__ __launch_bounds__(256) void unpad_rows_kernel(const uint16_t* __restrict__ src, uint16_t* __restrict__ dst,
+                                                         long long rows, int c, int cp) {
+  const int groups = cp / 8;
+  const long long n = rows * groups;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+    const long long r = i / groups;
+    const int d = (int)(i - r * groups) * 8;
+    const uint16_t* s = src + (size_t)r * (size_t)cp + d;
+    uint16_t* t = dst + (size_t)r * (size_t)c + d;
+    if (d + 8 <= c) {
+      *(mi::Pack<uint16_t>*)t = mi::load_pack(s);
+    } else {
+      for (int k = 0; d + k < c; ++k) t[k] = s[k];
+    }
+  }
+}
+
 // dst[c][0, rp) = src[0, rows)[c], then zeros: an operand whose rows are
 // contracted, turned.  64 x 64 pieces through LDS.
 __global__ __launch_bounds__(256) void turn_rows_kernel(const uint16_t* __restrict__ src, uint16_t* __restrict__ dst,
@@ -423,13 +441,24 @@ int fwd_plan(const mi_epilogue_args* a, const mi_tile_cfg* cfg, char* ws, Fwd* f
   return prc;
 }
 
+// Whether a weight's gradient whose rows do not start on 16 bytes comes from
+// a product of the turned operand, which stores where it belongs, rather than
+// from padded rows and a copy of them.  Of rhs [K,N] it always does: lhs is
+// turned and not padded (us turned and copied, M x N x K: 16 x 8001 x 12345 71
+// and 127, 1000 x 1501 x 777 23.4 and 23.6, 4000 x 3001 x 2001 80 and 88).  Of
+// rhs [N,K] dpre is turned next to lhs's padded copy, which only a result
+// larger than its operands pays for: 75 and 126, 31 and 23, 94 and 83; 100 x
+// 5001 x 1503 23.3 and 25.4, 16 x 1001 x 1001 13.6 and 12.
+bool better_turned(int M, int N, int K, bool bt) { return !bt || (M <= 256 && (long long)N * K >= 4 << 20); }
+
 struct Bwd {
   Padded dout, lhs, rhs;      // dout: dpre's place, or dout's padded copy
   bool dpre;                  // dout * act'(pre) goes to that place
   Product dlhs, drhs;
   bool turned;                // drhs by a product of its turned operand (else mi_matmul_lhsT_rhs_bf16)
-  size_t dlhs_part, drhs_part, turn_at, bias_at, bytes;
-  int chunks, rp;
+  bool copied;                // that product's result goes through padded rows
+  size_t dlhs_part, drhs_part, turn_at, drhs_at, bias_at, bytes;
+  int chunks, rp, kp;
 };
 int bwd_plan(const mi_epilogue_grad_args* a, char* ws, Bwd* b) {
   const int rc = check_sizes(a->M, a->N, a->K, a->activation);
@@ -475,9 +504,13 @@ int bwd_plan(const mi_epilogue_grad_args* a, char* ws, Bwd* b) {
   }
   if (a->drhs) {
     // The lhsT.rhs product stores whole 16-byte pieces of rows.  Other results
-    // take the operand whose columns are the result's rows turned, and the
-    // epilogue product of it: drhs[K,N] = (lhs^T) . dpre, drhs[N,K] = (dpre^T) . lhs.
-    b->turned = K % 8 != 0 || N % 8 != 0 || !at16(a->drhs);
+    // go through padded rows and are copied from there, or take the operand
+    // whose columns are the result's rows turned and the epilogue product of
+    // it: drhs[K,N] = (lhs^T) . dpre, drhs[N,K] = (dpre^T) . lhs.
+    const bool odd = K % 8 != 0 || N % 8 != 0 || !at16(a->drhs);
+    b->turned = odd && better_turned(a->M, N, K, bt);
+    b->copied = odd && !b->turned;
+    b->kp = up8(K);
     if (!b->turned || bt) b->lhs = padded(a->lhs, M, K, &b->bytes);
     const uint16_t* lhs = placed(a->lhs, ws, b->lhs);
     if (b->turned) {
@@ -489,8 +522,9 @@ int bwd_plan(const mi_epilogue_grad_args* a, char* ws, Bwd* b) {
       b->drhs_part = take(b->drhs.ws_bytes);
     } else {
       // Its operands, and its loads past their ends.
-      const unsigned long long span = ((unsigned long long)M + 1024) * (unsigned long long)(K > N ? K : N) * 2ull;
+      const unsigned long long span = ((unsigned long long)M + 1024) * (unsigned long long)up8(K > N ? K : N) * 2ull;
       if (span > kMaxOffset) return fail(MI_E_RANGE, "operand spans exceed 32-bit buffer offsets (%llu bytes)", span);
+      if (b->copied) b->drhs_at = take((size_t)b->kp * up8(N) * 2);
     }
   }
   return MI_OK;
@@ -658,8 +692,14 @@ int mi_matmul_epilogue_backward_bf16(const mi_epilogue_grad_args* a, void* works
   if (a->drhs) {
     // drhs[K,N] = lhs^T . dpre, or drhs[N,K] = dpre^T . lhs: rows M contracted.
     const uint16_t* lhs = placed(a->lhs, ws, b.lhs);
-    return bt ? mi::capi::matmul_lhsT_rhs_bf16(dpre, lhs, a->drhs, N, K, M, nullptr, stream, nullptr, 0)
-              : mi::capi::matmul_lhsT_rhs_bf16(lhs, dpre, a->drhs, K, N, M, nullptr, stream, nullptr, 0);
+    void* out = b.copied ? (void*)(ws + b.drhs_at) : a->drhs;
+    rc = bt ? mi::capi::matmul_lhsT_rhs_bf16(dpre, lhs, out, np, b.kp, M, nullptr, stream, nullptr, 0)
+            : mi::capi::matmul_lhsT_rhs_bf16(lhs, dpre, out, b.kp, np, M, nullptr, stream, nullptr, 0);
+    if (rc != MI_OK || !b.copied) return rc;
+    const long long rows = bt ? N : K;
+    const int c = bt ? K : N;
+    unpad_rows_kernel<<<dim3(blocks_for(rows * (up8(c) / 8))), dim3(256), 0, s>>>((const uint16_t*)out, (uint16_t*)a->drhs, rows, c, up8(c));
+    return launched("gradient's copy");
   }
   return MI_OK;
 }

@@ -51,7 +51,7 @@ def test_shapes(gpu, M, N, K, transposed):
 @pytest.mark.parametrize("transposed", [False, True])
 @pytest.mark.parametrize("M,N,K", [(1, 8, 8), (1, 9, 1000), (2, 4097, 71), (31, 129, 65), (32, 128, 127), (33, 8, 9),
                                    (40, 1001, 2049), (64, 65, 4099), (100, 200, 201), (256, 300, 333), (257, 300, 333),
-                                   (600, 77, 90), (5, 7, 100), (5, 100, 7)])
+                                   (600, 77, 90), (5, 7, 100), (5, 100, 7), (9, 2051, 2049)])
 def test_odd_sizes_as_they_are_and_copied(gpu, M, N, K, transposed):
     """Rows that do not start on 16 bytes: few of them go through registers (whole and partial pieces, tiles and parts),
     more are copied to padded ones; aligned sizes at odd addresses too, and infinities that must not leave the last
