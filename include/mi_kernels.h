@@ -250,7 +250,7 @@ enum { MI_DTYPE_BF16 = 0, MI_DTYPE_F16 = 1, MI_DTYPE_F32 = 2 };
  * in fp32, one rounding to y's type (x's).  Rows of x are ldx elements apart
  * (0: every row the same), y is contiguous.  weight, bias [D]: of x's type,
  * or fp32 (params_f32); NULL for 1 and 0.  mean, rstd [rows] fp32: what the
- * gradient takes; NULL where not wanted.  rows may be 0; any D > 0. */
+ * gradient takes; NULL where not wanted.  rows may be 0; D from 1 to 2^28. */
 typedef struct {
   const void *x, *weight, *bias;
   void* y;
@@ -283,14 +283,15 @@ int mi_layer_norm_backward(const mi_layer_norm_grad_args* args, void* workspace,
  * [N] bf16, or fp32 (bias_f32); residual, out, pre [M,N]; all contiguous.
  * bias, residual: NULL for none.  pre: NULL, or gets lhs . rhs + bias, which
  * the gradient takes.  Any M, N, K >= 0 (K = 0: a product of 0); operands
- * under 4 GiB (MI_E_RANGE).  Operands whose rows do not start on 16 bytes
- * (K or, untransposed, N no multiple of 8) are copied to padded rows in the
- * workspace first.
+ * under 4 GiB, sizes under 2^31 - 2^20 (MI_E_RANGE).  Operands whose rows do
+ * not start on 16 bytes (K or, untransposed, N no multiple of 8, or the
+ * pointer off 16) are read as they are by up to 256 rows of lhs, and by more,
+ * or with a cfg, from padded copies in the workspace.
  *
  * cfg: block_m, block_n, block_k, waves, lds_stages and variant (1: rhs read
  * non-temporally, for few rows) of one of mi_epilogue_config's, split_k
- * 1..16 (every part at least one K tile) and group_m (0: 8); NULL: the
- * library's choice for the shape. */
+ * 1..16 (every part at least one K tile; 1 where N > 2^20) and group_m (0:
+ * 8); NULL: the library's choice for the shape. */
 enum { MI_ACT_NONE = 0, MI_ACT_RELU = 1, MI_ACT_GELU = 2, MI_ACT_GELU_TANH = 3, MI_ACT_SILU = 4 };
 typedef struct {
   const void *lhs, *rhs, *bias, *residual;
@@ -309,8 +310,7 @@ int mi_matmul_epilogue_bf16(const mi_epilogue_args* args, const mi_tile_cfg* cfg
  * rounded to bf16, the type of the matrix cores' operands; dbias = sum_m dpre
  * takes it unrounded and has the bias's type.  The residual's gradient is
  * dout itself.  pre: what the forward call wrote (NULL for MI_ACT_NONE).
- * Each output NULL where not wanted.  drhs's product may take split-K
- * workspace as mi_matmul_lhsT_rhs_bf16 does. */
+ * Each output NULL where not wanted; dbias of at most 2^28 columns. */
 typedef struct {
   const void *dout, *lhs, *rhs, *pre;
   void *dlhs, *drhs, *dbias;
@@ -325,8 +325,9 @@ int mi_matmul_epilogue_backward_bf16(const mi_epilogue_grad_args* args, void* wo
  * (||grad||_F + eps), turned where m > n; then steps times A = X X^T, X =
  * a X + (b A + c A A) X.  The iterates are held in 16 bits of mantissa (two
  * bf16) and the products accumulate in fp32.  Any sizes; a matrix's planes
- * (4 bytes an element, the longer side rounded up to 64) under 4 GiB,
- * at most 65535 matrices (MI_E_RANGE). */
+ * (4 bytes an element, the longer side rounded up to 32, 512 rows more than
+ * the shorter has) under 4 GiB, no side over 2^20, at most 65535 matrices
+ * (MI_E_RANGE). */
 typedef struct {
   const void* grad;
   void* out;

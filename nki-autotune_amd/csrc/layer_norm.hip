@@ -10,16 +10,14 @@ using mi::ColumnSum;
 using mi::Fp16;
 using mi::LnBwd;
 using mi::LnFwd;
+using mi::capi::check_overlap;
 using mi::capi::fail;
+using mi::capi::Range;
 
 constexpr long long kMaxGrid = 1 << 20;  // blocks of one launch; they walk over the rows
 constexpr int kLongChunks = 256;         // row chunks of the column sums of long rows
 
 size_t elem_size(int dtype) { return dtype == MI_DTYPE_F32 ? 4 : 2; }
-
-bool overlap(const void* p, size_t pb, const void* q, size_t qb) {
-  return p && q && pb && qb && (uintptr_t)p < (uintptr_t)q + qb && (uintptr_t)q < (uintptr_t)p + pb;
-}
 
 // Bytes from the first to past the last element of `rows` rows of D, a row stride of ld.
 size_t span(long long rows, long long ld, int D, size_t elem) {
@@ -114,7 +112,7 @@ void bwd_run(const LnBwd& p, const BwdPlan& b, hipStream_t s) {
 
 int check_common(long long rows, int D, long long ldx, int dtype) {
   if (rows < 0 || D <= 0) return fail(MI_E_ARGS, "bad size rows=%lld D=%d (D must be positive)", rows, D);
-  if (D > 1 << 30) return fail(MI_E_RANGE, "D=%d over %d", D, 1 << 30);
+  if (D > 1 << 28) return fail(MI_E_RANGE, "D=%d over %d", D, 1 << 28);  // one launch adds up the parameters' gradients
   if (ldx < 0) return fail(MI_E_ARGS, "negative row stride %lld", ldx);
   if (dtype != MI_DTYPE_BF16 && dtype != MI_DTYPE_F16 && dtype != MI_DTYPE_F32)
     return fail(MI_E_ARGS, "unknown dtype %d", dtype);
@@ -138,9 +136,10 @@ int mi_layer_norm(const mi_layer_norm_args* a, void* stream) {
       (uintptr_t)a->mean % 4 || (uintptr_t)a->rstd % 4)
     return fail(MI_E_ALIGN, "a pointer is not aligned to its elements");
   const size_t yb = (size_t)a->rows * D * es, sb = (size_t)a->rows * 4;
-  if (overlap(a->y, yb, a->x, span(a->rows, a->ldx, a->D, es)) || overlap(a->y, yb, a->weight, D * ps) ||
-      overlap(a->y, yb, a->bias, D * ps) || overlap(a->y, yb, a->mean, sb) || overlap(a->y, yb, a->rstd, sb))
-    return fail(MI_E_ARGS, "y overlaps another operand");
+  const Range in[] = {{a->x, span(a->rows, a->ldx, a->D, es)}, {a->weight, D * ps}, {a->bias, D * ps}},
+              out[] = {{a->y, yb}, {a->mean, sb}, {a->rstd, sb}};
+  const int orc = check_overlap(out, in);
+  if (orc != MI_OK) return orc;
   const LnFwd p = {a->x, a->weight, a->bias, a->y, a->mean, a->rstd, a->rows, a->ldx, a->D, a->eps, a->params_f32 != 0};
   const hipStream_t s = (hipStream_t)stream;
   if (a->dtype == MI_DTYPE_BF16) fwd_run<Bf16>(p, s);
@@ -173,21 +172,11 @@ int mi_layer_norm_backward(const mi_layer_norm_grad_args* a, void* workspace, un
       (uintptr_t)a->dweight % ps || (uintptr_t)a->dbias % ps || (uintptr_t)a->mean % 4 || (uintptr_t)a->rstd % 4)
     return fail(MI_E_ALIGN, "a pointer is not aligned to its elements");
   const size_t D = (size_t)a->D, sb = (size_t)a->rows * 4;
-  const struct {
-    const void* p;
-    size_t n;
-  } in[] = {{a->x, span(a->rows, a->ldx, a->D, es)},
-            {a->dout, span(a->rows, a->lddout, a->D, es)},
-            {a->weight, D * ps},
-            {a->mean, sb},
-            {a->rstd, sb}},
-    out[] = {{a->dx, (size_t)a->rows * D * es}, {a->dweight, D * ps}, {a->dbias, D * ps}, {workspace, (size_t)need}};
-  for (int i = 0; i < 4; ++i) {
-    for (const auto& q : in)
-      if (overlap(out[i].p, out[i].n, q.p, q.n)) return fail(MI_E_ARGS, "an output overlaps an input");
-    for (int j = 0; j < i; ++j)
-      if (overlap(out[i].p, out[i].n, out[j].p, out[j].n)) return fail(MI_E_ARGS, "two outputs overlap");
-  }
+  const Range in[] = {{a->x, span(a->rows, a->ldx, a->D, es)}, {a->dout, span(a->rows, a->lddout, a->D, es)},
+                      {a->weight, D * ps}, {a->mean, sb}, {a->rstd, sb}},
+              out[] = {{a->dx, (size_t)a->rows * D * es}, {a->dweight, D * ps}, {a->dbias, D * ps}, {workspace, (size_t)need}};
+  const int orc = check_overlap(out, in);
+  if (orc != MI_OK) return orc;
   const hipStream_t s = (hipStream_t)stream;
   if (a->rows == 0) {
     // No row to read (the kernels take at least one): the sums are 0.

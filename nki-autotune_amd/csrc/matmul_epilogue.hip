@@ -12,9 +12,11 @@ using mi::AnyMM;
 using mi::EpiEntry;
 using mi::EpiMM;
 using mi::EpiOut;
+using mi::capi::check_overlap;
 using mi::capi::fail;
 using mi::capi::kMaxOffset;
 using mi::capi::kMaxSplit;
+using mi::capi::Range;
 
 // ---- kernels beside the products --------------------------------------
 
@@ -215,25 +217,6 @@ int up8(int v) { return (v + 7) / 8 * 8; }
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 bool at16(const void* p) { return (uintptr_t)p % 16 == 0; }
 
-bool overlap(const void* p, size_t pb, const void* q, size_t qb) {
-  return p && q && pb && qb && (uintptr_t)p < (uintptr_t)q + qb && (uintptr_t)q < (uintptr_t)p + pb;
-}
-struct Range {
-  const void* p;
-  size_t n;
-};
-// No output shares a byte with an input or another output.
-template <size_t NO, size_t NI>
-int check_overlap(const Range (&out)[NO], const Range (&in)[NI]) {
-  for (size_t i = 0; i < NO; ++i) {
-    for (const Range& q : in)
-      if (overlap(out[i].p, out[i].n, q.p, q.n)) return fail(MI_E_ARGS, "an output overlaps an input");
-    for (size_t j = 0; j < i; ++j)
-      if (overlap(out[i].p, out[i].n, out[j].p, out[j].n)) return fail(MI_E_ARGS, "two outputs overlap");
-  }
-  return MI_OK;
-}
-
 const EpiEntry* table(bool bt, int* n) { return bt ? mi::epi_table_nt(n) : mi::epi_table_nn(n); }
 
 const EpiEntry* find(bool bt, const mi_tile_cfg& c) {
@@ -404,7 +387,7 @@ const uint16_t* placed(const void* src, char* ws, const Padded& q) {
 
 int check_sizes(int M, int N, int K, int act) {
   if (M < 0 || N < 0 || K < 0) return fail(MI_E_ARGS, "negative size M=%d N=%d K=%d", M, N, K);
-  constexpr int most = 0x7FFFFFFF - 1024;  // sizes are rounded up to blocks in 32 bits
+  constexpr int most = 0x7FFFFFFF - (1 << 20);  // indexes run a grid's stride past a size in 32 bits
   if (M > most || N > most || K > most) return fail(MI_E_RANGE, "a size over %d (M=%d N=%d K=%d)", most, M, N, K);
   if (act < MI_ACT_NONE || act > MI_ACT_SILU) return fail(MI_E_ARGS, "unknown activation %d", act);
   const unsigned long long lim = kMaxOffset / 2;
@@ -457,6 +440,8 @@ struct Bwd {
   Product dlhs, drhs;
   bool turned;                // drhs by a product of its turned operand (else mi_matmul_lhsT_rhs_bf16)
   bool copied;                // that product's result goes through padded rows
+  mi_tile_cfg lhsT;           // its config, and the workspace of it
+  size_t lhsT_bytes;
   size_t dlhs_part, drhs_part, turn_at, drhs_at, bias_at, bytes;
   int chunks, rp, kp;
 };
@@ -474,6 +459,7 @@ int bwd_plan(const mi_epilogue_grad_args* a, char* ws, Bwd* b) {
     return at;
   };
   if (a->dbias) {
+    if (N > 1 << 28) return fail(MI_E_RANGE, "dbias of %d columns, over %d", N, 1 << 28);  // one launch adds them up
     const int xb = (up8(N) + 511) / 512;
     const int rows4 = (a->M + 3) / 4, want = 2048 / xb;
     b->chunks = want < 1 ? 1 : want > 256 ? 256 : want;
@@ -525,6 +511,10 @@ int bwd_plan(const mi_epilogue_grad_args* a, char* ws, Bwd* b) {
       const unsigned long long span = ((unsigned long long)M + 1024) * (unsigned long long)up8(K > N ? K : N) * 2ull;
       if (span > kMaxOffset) return fail(MI_E_RANGE, "operand spans exceed 32-bit buffer offsets (%llu bytes)", span);
       if (b->copied) b->drhs_at = take((size_t)b->kp * up8(N) * 2);
+      const int rows = bt ? up8(N) : b->kp, cols = bt ? b->kp : up8(N);
+      mi::capi::pick_default(MI_KERNEL_MATMUL_LHST_RHS_BF16, rows, cols, a->M, &b->lhsT);
+      b->lhsT_bytes = mi::workspace_bytes(MI_KERNEL_MATMUL_LHST_RHS_BF16, b->lhsT, rows, cols, a->M, mi::capi::device_cus());
+      if (b->lhsT_bytes) b->drhs_part = take(b->lhsT_bytes + 256);  // 256: it starts on so many
     }
   }
   return MI_OK;
@@ -693,8 +683,9 @@ int mi_matmul_epilogue_backward_bf16(const mi_epilogue_grad_args* a, void* works
     // drhs[K,N] = lhs^T . dpre, or drhs[N,K] = dpre^T . lhs: rows M contracted.
     const uint16_t* lhs = placed(a->lhs, ws, b.lhs);
     void* out = b.copied ? (void*)(ws + b.drhs_at) : a->drhs;
-    rc = bt ? mi::capi::matmul_lhsT_rhs_bf16(dpre, lhs, out, np, b.kp, M, nullptr, stream, nullptr, 0)
-            : mi::capi::matmul_lhsT_rhs_bf16(lhs, dpre, out, b.kp, np, M, nullptr, stream, nullptr, 0);
+    char* part = b.lhsT_bytes ? (char*)(((uintptr_t)ws + b.drhs_part + 255) / 256 * 256) : nullptr;
+    rc = bt ? mi::capi::matmul_lhsT_rhs_bf16(dpre, lhs, out, np, b.kp, M, &b.lhsT, stream, part, b.lhsT_bytes, false)
+            : mi::capi::matmul_lhsT_rhs_bf16(lhs, dpre, out, b.kp, np, M, &b.lhsT, stream, part, b.lhsT_bytes, false);
     if (rc != MI_OK || !b.copied) return rc;
     const long long rows = bt ? N : K;
     const int c = bt ? K : N;

@@ -438,11 +438,11 @@ int run_kept(const mi::MiEntry* e, const mi_tile_cfg& cfg, const mi::MiArgs& a, 
 }
 
 // fixed_ws != NULL: the caller's device buffer of fixed_cap bytes serves as
-// the workspace (nothing is allocated; a larger need is rejected); its
-// stream-K counters must be 0 (a static array, zero when loaded; every
-// stream-K launch leaves them 0).
+// the workspace (nothing is allocated; a larger need is rejected).
+// fixed_zeroed: its stream-K counters are 0 (a static array, zero when
+// loaded; every stream-K launch leaves them 0).
 int run(int kernel_id, const mi_tile_cfg* cfg_in, const mi::MiArgs& args_in, void* stream, char* fixed_ws = nullptr,
-        size_t fixed_cap = 0) {
+        size_t fixed_cap = 0, bool fixed_zeroed = true) {
   mi_tile_cfg cfg;
   const mi::MiEntry* e = nullptr;
   int rc = resolve(kernel_id, cfg_in, args_in, &cfg, &e);
@@ -455,7 +455,7 @@ int run(int kernel_id, const mi_tile_cfg* cfg_in, const mi::MiArgs& args_in, voi
     if (ws_bytes > fixed_cap)
       return fail(MI_E_RANGE, "the config needs %zu bytes of workspace, over the %zu-byte static scratch", ws_bytes,
                   fixed_cap);
-    return launch(e, cfg, a, fixed_ws, true, stream);
+    return launch(e, cfg, a, fixed_ws, fixed_zeroed, stream);
   }
   hipMemPool_t pool = nullptr;
   if ((rc = workspace_pool(&pool)) != MI_OK) return rc;
@@ -488,7 +488,7 @@ namespace mi {
 namespace capi {
 
 int matmul_lhsT_rhs_bf16(const void* lhsT, const void* rhs, void* out, int M, int N, int K, const mi_tile_cfg* cfg,
-                         void* stream, char* fixed_ws, size_t fixed_cap) {
+                         void* stream, char* fixed_ws, size_t fixed_cap, bool fixed_zeroed) {
   if (M < 0 || N < 0 || K < 0) return fail(MI_E_ARGS, "negative size M=%d N=%d K=%d", M, N, K);
   if (M == 0 || N == 0) return MI_OK;
   if (!out) return fail(MI_E_ARGS, "null output pointer");
@@ -502,7 +502,7 @@ int matmul_lhsT_rhs_bf16(const void* lhsT, const void* rhs, void* out, int M, in
   if (overlaps(out, ob, lhsT, (size_t)K * M * 2) || overlaps(out, ob, rhs, (size_t)K * N * 2))
     return fail(MI_E_ARGS, "out overlaps an input");
   mi::MiArgs a = {lhsT, rhs, nullptr, out, M, N, K, 0.0f, 0.0f, 8};
-  return run(MI_KERNEL_MATMUL_LHST_RHS_BF16, cfg, a, stream, fixed_ws, fixed_cap);
+  return run(MI_KERNEL_MATMUL_LHST_RHS_BF16, cfg, a, stream, fixed_ws, fixed_cap, fixed_zeroed);
 }
 
 }  // namespace capi

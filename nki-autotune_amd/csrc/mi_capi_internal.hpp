@@ -25,6 +25,26 @@ inline unsigned long long f32_kw_span(int cols, int K, int block) {
 // returns `code`.
 int fail(int code, const char* fmt, ...);
 
+// Bytes that a call reads or writes.  No output (NULL or empty: none) shares
+// one with an input or another output.
+struct Range {
+  const void* p;
+  size_t n;
+};
+inline bool overlap(const Range& a, const Range& b) {
+  return a.p && b.p && a.n && b.n && (uintptr_t)a.p < (uintptr_t)b.p + b.n && (uintptr_t)b.p < (uintptr_t)a.p + a.n;
+}
+template <size_t NO, size_t NI>
+int check_overlap(const Range (&out)[NO], const Range (&in)[NI]) {
+  for (size_t i = 0; i < NO; ++i) {
+    for (const Range& q : in)
+      if (overlap(out[i], q)) return fail(MI_E_ARGS, "an output overlaps an input");
+    for (size_t j = 0; j < i; ++j)
+      if (overlap(out[i], out[j])) return fail(MI_E_ARGS, "two outputs overlap");
+  }
+  return MI_OK;
+}
+
 // The prebuilt instance of `kernel_id` for cfg's tile parameters and
 // variant (split_k and group_m aside), or NULL.
 const MiEntry* find(int kernel_id, const mi_tile_cfg& cfg);
@@ -46,9 +66,10 @@ int pick_default_no_gamma(int M, int N, int K, mi_tile_cfg* cfg);
 // The body of mi_matmul_lhsT_rhs_bf16.  fixed_ws == NULL: a call that needs
 // device workspace takes it from the library's stream-ordered pool;
 // otherwise fixed_ws (fixed_cap bytes, 256-byte aligned) is the workspace
-// and a config needing more is rejected with MI_E_RANGE.
+// and a config needing more is rejected with MI_E_RANGE.  fixed_zeroed: the
+// stream-K counters at its start are known to be 0.
 int matmul_lhsT_rhs_bf16(const void* lhsT, const void* rhs, void* out, int M, int N, int K, const mi_tile_cfg* cfg,
-                         void* stream, char* fixed_ws, size_t fixed_cap);
+                         void* stream, char* fixed_ws, size_t fixed_cap, bool fixed_zeroed = true);
 
 }  // namespace capi
 }  // namespace mi

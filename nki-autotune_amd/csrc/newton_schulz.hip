@@ -235,12 +235,8 @@ int mi_newton_schulz(const mi_newton_schulz_args* args, void* workspace, unsigne
   if (!workspace || workspace_bytes < q.bytes || (uintptr_t)workspace % 16)
     return fail(MI_E_ARGS, "the call needs %zu bytes of workspace, 16-byte aligned", q.bytes);
   if ((uintptr_t)args->grad % es || (uintptr_t)args->out % 2) return fail(MI_E_ALIGN, "a pointer is not aligned to its elements");
-  const auto overlap = [](const void* a, size_t ab, const void* b, size_t bb) {
-    return (uintptr_t)a < (uintptr_t)b + bb && (uintptr_t)b < (uintptr_t)a + ab;
-  };
-  if (overlap(args->grad, total * es, args->out, total * 2) || overlap(workspace, q.bytes, args->grad, total * es) ||
-      overlap(workspace, q.bytes, args->out, total * 2))
-    return fail(MI_E_ARGS, "out overlaps grad, or the workspace one of them");
+  const mi::capi::Range in[] = {{args->grad, total * es}}, outs[] = {{args->out, total * 2}, {workspace, q.bytes}};
+  if ((rc = mi::capi::check_overlap(outs, in)) != MI_OK) return rc;
   const hipStream_t st = (hipStream_t)stream;
   char* ws = (char*)workspace;
   double* part = (double*)(ws + q.part);

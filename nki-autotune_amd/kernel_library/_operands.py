@@ -25,6 +25,8 @@ def tensor(name: str, t: object, dtypes: Container[torch.dtype], ref: torch.Tens
         raise ValueError(f"{name} must live on a HIP device (got {t.device})")
     if t.dtype not in dtypes:
         raise ValueError(f"{name} dtype {t.dtype} not in {tuple(dtypes)}")
+    if t.is_neg():
+        raise ValueError(f"{name} is a negated view: its memory holds other values (resolve_neg() first)")
     if ref is not None and t.device != ref.device:
         raise ValueError(f"{name} is on {t.device}, {ref_name} on {ref.device}: all operands must share a device")
 

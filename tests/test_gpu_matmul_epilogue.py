@@ -311,7 +311,8 @@ def test_same_bits_on_streams_and_in_graphs(gpu):
     import kernel_library as kl
 
     # Split-K, padded operands and the plain path, forward and backward.
-    for M, N, K, transposed in ((40, 520, 2048, False), (70, 131, 333, True), (512, 512, 256, False)):
+    for M, N, K, transposed in ((40, 520, 2048, False), (70, 131, 333, True), (512, 512, 256, False), (4096, 128, 136, False),
+                                (4095, 129, 128, True)):
         lhs, rhs, b, r = _inputs(M, N, K, gpu, transposed)
         pre = torch.empty(M, N, dtype=torch.bfloat16, device=gpu)
 

@@ -52,6 +52,8 @@ def _ln(**kw):
     (dict(y=_at(0) - 2), _lib.MI_E_ARGS),
     (dict(y=_at(1) + 2), _lib.MI_E_ARGS),
     (dict(y=_at(5)), _lib.MI_E_ARGS),
+    (dict(mean=_at(0)), _lib.MI_E_ARGS),
+    (dict(rstd=_at(4)), _lib.MI_E_ARGS),
     (dict(rows=0, x=None, y=None), _lib.MI_OK),
 ])
 def test_layer_norm(kw, code):
@@ -79,6 +81,7 @@ def _ln_bwd(**kw):
     (dict(dweight=_at(2)), _lib.MI_E_ARGS),
     (dict(dx=_at(9)), _lib.MI_E_ARGS),  # the workspace
     (dict(dx=None, dweight=None, dbias=None), _lib.MI_OK),
+    (dict(D=(1 << 28) + 1), _lib.MI_E_RANGE),
 ])
 def test_layer_norm_backward(kw, code):
     L = _lib.lib()
@@ -118,6 +121,7 @@ BIG = 2**31 - 1
     (dict(M=BIG, N=BIG, K=0), _lib.MI_E_RANGE),
     (dict(M=1, N=BIG, K=1), _lib.MI_E_RANGE),
     (dict(M=1, N=1, K=BIG), _lib.MI_E_RANGE),
+    (dict(M=BIG - (1 << 20) + 1, N=1, K=0), _lib.MI_E_RANGE),
     (dict(lhs=None), _lib.MI_E_ARGS),
     (dict(out=None), _lib.MI_E_ARGS),
     (dict(lhs=_at(0) + 1), _lib.MI_E_ALIGN),
@@ -193,6 +197,8 @@ def _mm_bwd(**kw):
     (dict(lhs=None), _lib.MI_E_ARGS),
     (dict(M=1 << 20, N=1 << 14), _lib.MI_E_RANGE),
     (dict(M=1 << 20, N=1 << 14, dlhs=None), _lib.MI_E_RANGE),
+    (dict(M=BIG - (1 << 20) + 1, N=1, K=0), _lib.MI_E_RANGE),
+    (dict(M=1, N=(1 << 28) + 1, K=0), _lib.MI_E_RANGE),
     (dict(dout=_at(0) + 1), _lib.MI_E_ALIGN),
     (dict(dbias=_at(6) + 2, bias_f32=1), _lib.MI_E_ALIGN),
     (dict(dlhs=_at(1)), _lib.MI_E_ARGS),
