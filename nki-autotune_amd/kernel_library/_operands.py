@@ -31,6 +31,13 @@ def tensor(name: str, t: object, dtypes: Container[torch.dtype], ref: torch.Tens
         raise ValueError(f"{name} is on {t.device}, {ref_name} on {ref.device}: all operands must share a device")
 
 
+def int32(**values: int) -> None:
+    """The values that a C int takes (ctypes would cut them to it)."""
+    for name, v in values.items():
+        if not -2**31 <= v < 2**31:
+            raise ValueError(f"{name}={v} does not fit 32 bits")
+
+
 def _span(t: torch.Tensor) -> tuple[int, int]:
     """The first byte of ``t`` and the one past its last."""
     if t.numel() == 0:

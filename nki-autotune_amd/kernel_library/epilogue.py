@@ -19,7 +19,7 @@ import ctypes
 import torch
 
 from kernel_library import _lib
-from kernel_library._operands import launch, no_overlap, tensor, workspace
+from kernel_library._operands import int32, launch, no_overlap, tensor, workspace
 from kernel_library.config import TileConfig, _torch_call
 
 _ACTIVATIONS = {None: _lib.MI_ACT_NONE, "none": _lib.MI_ACT_NONE, "relu": _lib.MI_ACT_RELU, "gelu": _lib.MI_ACT_GELU,
@@ -44,6 +44,7 @@ def _operands(lhs: torch.Tensor, rhs: torch.Tensor, rhs_transposed: bool) -> tup
     N, K2 = rhs.shape if rhs_transposed else rhs.shape[::-1]
     if K != K2:
         raise ValueError(f"contraction mismatch: lhs has K={K}, rhs has K={K2}")
+    int32(M=M, N=N, K=K)
     return M, N, K
 
 

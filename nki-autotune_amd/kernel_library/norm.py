@@ -17,7 +17,7 @@ import ctypes
 import torch
 
 from kernel_library import _lib
-from kernel_library._operands import launch, no_overlap, tensor, workspace
+from kernel_library._operands import int32, launch, no_overlap, tensor, workspace
 from kernel_library.config import _torch_call
 
 _DTYPES = {torch.bfloat16: _lib.MI_DTYPE_BF16, torch.float16: _lib.MI_DTYPE_F16, torch.float32: _lib.MI_DTYPE_F32}
@@ -30,6 +30,7 @@ def _rows(name: str, t: torch.Tensor) -> tuple[int, int, int]:
     D = t.shape[-1]
     if D == 0:
         raise ValueError(f"{name} has rows of no elements, shape {tuple(t.shape)}")
+    int32(D=D)
     rows = t.numel() // D
     if t.is_contiguous():
         return rows, D, D

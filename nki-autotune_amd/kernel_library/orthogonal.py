@@ -14,7 +14,7 @@ import ctypes
 import torch
 
 from kernel_library import _lib
-from kernel_library._operands import launch, no_overlap, tensor, workspace
+from kernel_library._operands import int32, launch, no_overlap, tensor, workspace
 from kernel_library.config import _torch_call
 
 _DTYPES = {torch.bfloat16: _lib.MI_DTYPE_BF16, torch.float32: _lib.MI_DTYPE_F32}
@@ -45,6 +45,7 @@ def newton_schulz(
         raise ValueError(f"eps must be finite and >= 0, got {eps}")
     batch = grad.shape[0] if grad.dim() == 3 else 1
     m, n = grad.shape[-2:]
+    int32(steps=steps, batch=batch, m=m, n=n)
     if out is None:
         out = torch.empty(grad.shape, dtype=torch.bfloat16, device=grad.device)
     else:

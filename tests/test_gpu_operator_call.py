@@ -113,3 +113,34 @@ def test_a_library_error_is_raised_by_either(gpu):
     for _ in range(2):
         with pytest.raises(kl.epilogue._lib.KernelLibraryError, match="rc=5"):
             kl.matmul_epilogue(lhs, wide, out=out)
+
+
+def test_sizes_past_32_bits_are_refused(gpu):
+    """A size that a C int cannot hold is refused, not cut to the one it would become."""
+    import torch
+
+    import kernel_library as kl
+
+    big = 2**32 + 8
+    bf = dict(dtype=torch.bfloat16, device=gpu)
+    none, eight = torch.empty(0, big, **bf), torch.zeros(8, 0, **bf)
+    stats = torch.empty(0, device=gpu)
+    for call in (lambda: kl.layer_norm(none), lambda: kl.layer_norm_backward(none, none, stats, stats),
+                 lambda: kl.matmul_epilogue(none, none, rhs_transposed=True),
+                 lambda: kl.matmul_epilogue(torch.empty(big, 0, **bf), eight, rhs_transposed=True),
+                 lambda: kl.matmul_epilogue_backward(torch.empty(0, 0, **bf), none, none, rhs_transposed=True),
+                 lambda: kl.newton_schulz(none), lambda: kl.newton_schulz(none.reshape(big, 0, 1)),
+                 lambda: kl.newton_schulz(torch.zeros(4, 4, **bf), steps=2**32)):
+        with pytest.raises(ValueError, match="32 bits"):
+            call()
+
+
+def test_negated_views_are_refused(gpu):
+    import torch
+
+    import kernel_library as kl
+
+    v = torch.randn(8, 1, dtype=torch.complex64, device=gpu).conj().imag
+    assert v.is_neg()
+    with pytest.raises(ValueError, match="negated"):
+        kl.layer_norm(v)
