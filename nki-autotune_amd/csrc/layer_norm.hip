@@ -40,17 +40,26 @@ void fwd(const LnFwd& p, hipStream_t s) {
   else mi::layer_norm_kernel<T, E, L, ROWS, false, (E < 32)><<<grid, block, 0, s>>>(p);
 }
 
+// Values of a lane and lanes of a row.  16 values a lane past 128: fewer lanes
+// to sum over, and a second 16-byte load of bf16 in flight (us of 256 MB of
+// rows in and out, 16 values and 8 on twice the lanes: bf16 D = 256 100 and
+// 107, 512 101 and 112, 1024 99 and 130, 2048 97 and 120; 4096 108 and 116;
+// fp32 within 4 either way).  Up to 64, 8 lanes of 8: 99 and 151 with 16 lanes
+// at bf16 D = 64, 154 and 260 at 32; at 128 16 lanes of 8 take 96, 8 of 16 102.
+// Past 8192 the values still fit 1024 lanes and the row is read once: 16384
+// 110 and 186 in three passes, 28672 143 and 197.
 template <class T>
 void fwd_run(const LnFwd& p, hipStream_t s) {
   constexpr int V = 16 / (int)sizeof(T);
   const int D = p.D;
   const unsigned rows = (unsigned)(p.rows < kMaxGrid ? p.rows : kMaxGrid);
   if (D < V) mi::layer_norm_long_kernel<T, 64, 1><<<dim3(rows), dim3(64), 0, s>>>(p);
+  else if (D <= 64) fwd<T, 8, 8>(p, s);
   else if (D <= 128) fwd<T, 8, 16>(p, s);
-  else if (D <= 256) fwd<T, 8, 32>(p, s);
-  else if (D <= 512) fwd<T, 8, 64>(p, s);
+  else if (D <= 256) fwd<T, 16, 16>(p, s);
+  else if (D <= 512) fwd<T, 16, 32>(p, s);
   else if (D <= 1024) fwd<T, 16, 64>(p, s);
-  else if (D <= 2048) fwd<T, 8, 256>(p, s);
+  else if (D <= 2048) fwd<T, 16, 128>(p, s);
   else if (D <= 4096) fwd<T, 16, 256>(p, s);
   else if (D <= 8192) fwd<T, 16, 512>(p, s);
   else if (D <= 16384) fwd<T, 16, 1024>(p, s);
@@ -58,11 +67,17 @@ void fwd_run(const LnFwd& p, hipStream_t s) {
   else mi::layer_norm_long_kernel<T, 1024, V><<<dim3(rows), dim3(1024), 0, s>>>(p);
 }
 
-// Rows longer than this, or shorter than 16 bytes, are read more than once.
+// Rows longer than this, or shorter than 16 bytes, are read more than once
+// (bf16 D = 8192 152 us against 282, 16384 168 against 296, of 256 MB each of
+// x, dout and dx).
 int bwd_most(int dtype) { return dtype == MI_DTYPE_F32 ? 8192 : 16384; }
 
 // Lanes of a row and blocks of the gradient's kernel; each block leaves a row
-// of partial sums.
+// of partial sums.  8 values a lane wherever they do: a lane holds their column
+// sums beside them (16 on half the lanes: bf16 D = 256 to 4096 5 % slower, fp32
+// up to twice, and with 64 rows 9 us for 6).  Rows of up to 128 bytes take 8
+// lanes: bf16 D = 32 191 us and 333 with 16, 64 161 and 193; fp32 32 163 and 217,
+// but 64 162 and 158.
 struct BwdPlan {
   int lanes, blocks;
   bool is_long;
@@ -71,7 +86,7 @@ BwdPlan bwd_plan(long long rows, int D, int dtype) {
   BwdPlan b;
   const bool f32 = dtype == MI_DTYPE_F32;
   b.is_long = D > bwd_most(dtype) || D < (f32 ? 4 : 8);
-  b.lanes = D <= 128 ? 16 : D <= 256 ? 32 : D <= 512 ? 64 : D <= 1024 ? 128 : D <= 2048 ? 256 : D <= 4096 ? 512 : 1024;
+  b.lanes = D <= (f32 ? 32 : 64) ? 8 : D <= 128 ? 16 : D <= 256 ? 32 : D <= 512 ? 64 : D <= 1024 ? 128 : D <= 2048 ? 256 : D <= 4096 ? 512 : 1024;
   const int per_block = b.is_long ? 1 : 1024 / b.lanes;
   const long long need = (rows + per_block - 1) / per_block, most = b.is_long ? kLongChunks : mi::capi::device_cus();
   b.blocks = (int)(need < most ? (need > 0 ? need : 1) : most);
@@ -100,7 +115,8 @@ void bwd_run(const LnBwd& p, const BwdPlan& b, hipStream_t s) {
       if (p.part)
         mi::layer_norm_columns_kernel<T, V><<<dim3((unsigned)((D + 256 * V - 1) / (256 * V)), chunks), dim3(256), 0, s>>>(p);
     }
-  } else if (D <= 128) bwd<T, 8, 16>(p, b, s);
+  } else if (D <= 128 / (int)sizeof(T)) bwd<T, 8, 8>(p, b, s);
+  else if (D <= 128) bwd<T, 8, 16>(p, b, s);
   else if (D <= 256) bwd<T, 8, 32>(p, b, s);
   else if (D <= 512) bwd<T, 8, 64>(p, b, s);
   else if (D <= 1024) bwd<T, 8, 128>(p, b, s);

@@ -5,12 +5,13 @@
 //   BT = false: out = A . B, B[K,N] (N contiguous; transposing operand reads)
 //   BT = true:  out = A . B^T, B[N,K] (K contiguous, like A)
 //
-// The main loop is the pipelined core of mi_gemm.hpp (LDS-direct panel loads,
-// STAGES K tiles in flight, operands of the next MFMA step read while this
-// one runs, one barrier a K tile); here K tiles are 64 wide, so that a row of
-// a K-contiguous panel is a whole 128-byte line and each line is requested
-// once.  The MFMAs compute out^T per 32x32 tile: a lane ends with 4
-// consecutive columns of one row.
+// The main loop is pipelined as that of mi_gemm.hpp is (LDS-direct panel
+// loads, STAGES K tiles in flight, operands of the next MFMA step read while
+// this one runs); here K tiles are 64 wide, so that a row of a K-contiguous
+// panel is a whole 128-byte line and each line is requested once, and the
+// MFMAs are 16x16x32, which read and write half the accumulator registers per
+// flop that 32x32x16 do (8192^3 with bias and gelu: 775 us and 834).  They
+// compute out^T: a lane ends with 4 consecutive columns of one row.
 //
 // The epilogue turns each wave's accumulators in its own piece of LDS as
 // fp32 (32 rows of 64 columns at a time, wave-private: no barrier), so that a
@@ -18,6 +19,13 @@
 // and outputs is a 16-byte piece of a whole line, and the values are rounded
 // once, after the last operation.  Residual rows are requested before the
 // turn and arrive behind it.
+//
+// Measured on one MI355X, where the plain products of this library reach 1470
+// TFLOP/s at 8192^3: that size with bias, gelu_tanh and the kept
+// pre-activation 793 us, 1390 TFLOP/s (MFMAs busy 74 % of the time, the rest
+// mostly waits at the barriers); 1000 x 5000 x 4104 with a residual 57 us,
+// where 80 blocks of 256x256 or 320 of 128x128 leave units idle; 16 x 28672 x
+// 8192 with silu 88 us, 5.3 TB/s of weight.
 #pragma once
 #include <type_traits>
 
@@ -26,8 +34,8 @@
 
 namespace mi {
 
-// Operands as the kernel reads them.  K, lda and ldb are multiples of 8; a_bytes, b_bytes: what lies behind the pointers (reads past it
-// give 0).
+// Operands as the kernel reads them.  K, lda and ldb are multiples of 8;
+// a_bytes, b_bytes: what lies behind the pointers (reads past it give 0).
 struct EpiMM {
   const uint16_t *a, *b;
   uint32_t a_bytes, b_bytes;

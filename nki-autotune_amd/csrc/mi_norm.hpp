@@ -12,7 +12,7 @@
 //
 // Both passes read every row once: its E values per lane stay in registers
 // between the sums and the output, so the bytes that cross HBM are the
-// tensors' own.  A row belongs to L lanes (16 of a wave, a wave, or up to 16
+// tensors' own.  A row belongs to L lanes (8 of a wave to 16
 // waves).  Blocks walk over the rows with the parameters in registers and the
 // next row's loads in flight behind this row's work; the gradient's keep the
 // column sums of dweight and dbias in registers too (2 E a lane), add their
@@ -25,8 +25,12 @@
 // row's end, it takes the row's last 16 bytes, computes what the lanes that
 // own them compute, stores the same, and leaves them out of the row's sums;
 // rows past the last are the last one again, left out of the column sums.
-// Measured on one MI355X against a copy's 4.9 TB/s: see the launches in
-// layer_norm.hip.
+//
+// Bound by HBM: on one MI355X, where a large copy runs at 4.9 TB/s, 16384 x
+// 8192 bf16 takes 98 us forward (5.5 TB/s; caches hold the last writes) and
+// 16384 x 4096 backward 77 us (5.2 TB/s); at most of the odd sizes 0.8 to 0.95
+// of that.  Few rows are bound by latency: 8 x 4096 2.3 us.
+// Rows of 64 or fewer values are bound by the instructions of their sums.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <hip/hip_fp16.h>

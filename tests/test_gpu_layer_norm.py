@@ -9,7 +9,7 @@ from block_oracle import layer_norm_backward as ln_bwd64
 pytestmark = pytest.mark.gpu
 
 # A row per wave, a few waves per row, rows longer than registers hold; whole vectors and odd sizes.
-SIZES = [(1, 1), (1, 8), (3, 7), (5, 64), (9, 100), (4, 512), (33, 513), (2, 1024), (7, 1501), (17, 2048), (5, 2056),
+SIZES = [(1, 1), (1, 8), (3, 7), (300, 17), (700, 32), (257, 33), (5, 64), (9, 100), (4, 512), (33, 513), (2, 1024), (7, 1501), (17, 2048), (5, 2056),
          (3, 4096), (300, 777), (1, 4104), (2, 8192), (3, 8191), (2, 16384), (2, 16392), (1, 16383), (2, 32768), (1, 40001)]
 TYPES = [("bfloat16", "bfloat16"), ("bfloat16", "float32"), ("float16", "float16"), ("float32", "float32")]
 
