@@ -14,20 +14,34 @@ using mi::capi::fail;
 constexpr int kNormBlocks = 256;  // blocks of one matrix's sum of squares
 
 // part[z][block] = the sum of squares of a share of G_z, in 64 bits (the
-// squares of small gradients leave fp32's range).
+// squares of small gradients leave fp32's range).  16 bytes a load, at any
+// address; block 0 also has the last n % V values.  4096 x 4096 bf16: 15 us
+// (value by value 61).
 template <class T>
 __global__ __launch_bounds__(256) void ns_square_kernel(const T* __restrict__ g, double* __restrict__ part, long long n) {
   __shared__ double xs[4];
+  constexpr int V = mi::Pack<T>::V, U = 4;
   const T* p = g + (size_t)blockIdx.y * (size_t)n;
+  const long long packs = n / V, step = (long long)gridDim.x * 256;
   double s = 0.0;
-  constexpr int U = 8;
-  const long long step = (long long)gridDim.x * 256;
-  for (long long i0 = (long long)blockIdx.x * 256 + threadIdx.x; i0 < n; i0 += U * step) {
-    float v[U];
+  for (long long i0 = (long long)blockIdx.x * 256 + threadIdx.x; i0 < packs; i0 += U * step) {
+    mi::Pack<T> v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = i0 + u * step < n ? mi::to_f32(p[i0 + u * step]) : 0.0f;
+    for (int u = 0; u < U; ++u) v[u] = mi::load_pack(p + (i0 + u * step < packs ? i0 + u * step : i0) * V);
 #pragma unroll
-    for (int u = 0; u < U; ++u) s += (double)v[u] * (double)v[u];
+    for (int u = 0; u < U; ++u) {
+      if (i0 + u * step >= packs) break;
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const double x = (double)mi::to_f32(v[u].v[k]);
+        s += x * x;
+      }
+    }
+  }
+  const long long rest = packs * V + threadIdx.x;
+  if (blockIdx.x == 0 && rest < n) {
+    const double x = (double)mi::to_f32(p[rest]);
+    s += x * x;
   }
 #pragma unroll
   for (int k = 32; k > 0; k >>= 1) s += __shfl_xor(s, k);
@@ -52,6 +66,25 @@ __global__ __launch_bounds__(256) void ns_init_kernel(const NsInit p) {
   __shared__ float tile[64][65];
   __shared__ float scale_lds;
   const int tid = (int)threadIdx.x, z = (int)blockIdx.z;
+  const T* g = (const T*)p.g + (size_t)z * (size_t)p.m * (size_t)p.n;
+  const int r0 = (int)blockIdx.y * 64, c0 = (int)blockIdx.x * 64;  // of X
+  const int row0 = p.turn ? c0 : r0, col0 = p.turn ? r0 : c0;      // of G
+  // 8 values a load, at any address: two a thread, on their way while the
+  // parts are added up.
+  mi::Pack<T, 8> in[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int row = row0 + tid / 8 + 32 * j, col = col0 + tid % 8 * 8;
+    const T* at = g + (size_t)row * (size_t)p.n + col;
+    in[j] = mi::Pack<T, 8>{};
+    if (row < p.m && col + 8 <= p.n) {
+      in[j] = mi::load_pack<T, 8>(at);
+    } else if (row < p.m) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (col + k < p.n) in[j].v[k] = at[k];
+    }
+  }
   if (tid < 64) {
     // The parts' sum, in an order fixed by their number.
     double t[kNormBlocks / 64];
@@ -62,15 +95,15 @@ __global__ __launch_bounds__(256) void ns_init_kernel(const NsInit p) {
     for (int k = 32; k > 0; k >>= 1) sum += __shfl_xor(sum, k);
     if (tid == 0) scale_lds = (float)(1.0 / (__builtin_sqrt(sum) + (double)p.eps));
   }
-  const T* g = (const T*)p.g + (size_t)z * (size_t)p.m * (size_t)p.n;
-  const int r0 = (int)blockIdx.y * 64, c0 = (int)blockIdx.x * 64;  // of X
-  for (int i = tid; i < 64 * 64; i += 256) {
-    const int a = i / 64, b = i % 64;
-    const int row = (p.turn ? c0 : r0) + a, col = (p.turn ? r0 : c0) + b;  // of G
-    const float v = row < p.m && col < p.n ? mi::to_f32(g[(size_t)row * (size_t)p.n + col]) : 0.0f;
-    if (p.turn) tile[b][a] = v;
-    else tile[a][b] = v;
-  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int a = tid / 8 + 32 * j, b = tid % 8 * 8 + k;
+      const float v = mi::to_f32(in[j].v[k]);
+      if (p.turn) tile[b][a] = v;
+      else tile[a][b] = v;
+    }
   __syncthreads();
   const float scale = scale_lds;
   uint16_t* x = p.x + (size_t)z * (size_t)p.s * (size_t)(2 * p.lp);
@@ -98,19 +131,35 @@ __global__ __launch_bounds__(256) void ns_last_kernel(const uint16_t* __restrict
   const int tid = (int)threadIdx.x, z = (int)blockIdx.z;
   const int r0 = (int)blockIdx.y * 64, c0 = (int)blockIdx.x * 64;  // of out
   const uint16_t* src = x + (size_t)z * (size_t)s * (size_t)(2 * lp);
-  for (int i = tid; i < 64 * 64; i += 256) {
-    const int a = i / 64, b = i % 64;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int a = tid / 8 + 32 * j, b = tid % 8 * 8;
     const int row = (turn ? c0 : r0) + a, col = (turn ? r0 : c0) + b;  // of X
-    const bool in = row < s && col < lp;
-    const uint16_t v = in ? src[(size_t)row * (size_t)(2 * lp) + mi::ns_at(col)] : (uint16_t)0;
-    if (turn) tile[b][a] = v;
-    else tile[a][b] = v;
+    mi::Pack<uint16_t> v = {};
+    if (row < s && col < lp) v = mi::load_pack(src + (size_t)row * (size_t)(2 * lp) + mi::ns_at(col));
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (turn) tile[b + k][a] = v.v[k];
+      else tile[a][b + k] = v.v[k];
+    }
   }
   __syncthreads();
   uint16_t* dst = out + (size_t)z * (size_t)m * (size_t)n;
-  for (int i = tid; i < 64 * 64; i += 256) {
-    const int r = r0 + i / 64, c = c0 + i % 64;
-    if (r < m && c < n) dst[(size_t)r * (size_t)n + c] = tile[i / 64][i % 64];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int a = tid / 8 + 32 * j, b = tid % 8 * 8, r = r0 + a, c = c0 + b;
+    if (r >= m || c >= n) continue;
+    uint16_t* to = dst + (size_t)r * (size_t)n + c;
+    mi::Pack<uint16_t> v;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v.v[k] = tile[a][b + k];
+    if (c + 8 <= n) {
+      *(mi::Pack<uint16_t>*)to = v;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (c + k < n) to[k] = v.v[k];
+    }
   }
 }
 
