@@ -1,6 +1,8 @@
 // matmul_epilogue.hip -- mi_matmul_epilogue_bf16 and its gradient: argument
 // checks, the config a call takes, workspaces and launches (products:
 // mi_mm_epi.hpp).
+#include <cmath>
+
 #include "mi_capi_internal.hpp"
 #include "mi_epi_table.hpp"
 #include "mi_mm_any.hpp"
@@ -234,13 +236,15 @@ const EpiEntry* find(bool bt, const mi_tile_cfg& c) {
 // The library's choice of a config for a product of these sizes: the least
 // estimated time (mi_epi_table.hpp) over the configs and part counts.  The
 // busiest unit's blocks run one after the other, or share it; no product is
-// faster than its bytes at 5.4 TB/s; parts cost a second launch and their
-// fp32 products written and read.
+// faster than its bytes at 5.4 TB/s, and one whose rhs the last-level cache
+// does not hold nears the larger of its blocks' time and its bytes' as the two
+// part; parts cost a second launch and their fp32 products written and read.
 mi_tile_cfg pick(int M, int N, int K, bool bt) {
   int n = 0;
   const EpiEntry* t = table(bt, &n);
   const int cus = mi::capi::device_cus();
-  const double mem = 2.0 * ((double)N * K + (double)M * K + (double)M * N) / 5.4e6;
+  const double bytes = 2.0 * ((double)N * K + (double)M * K + (double)M * N);
+  const bool streamed = 2.0 * (double)N * K > 256.0 * (1 << 20);
   const int kt = (K + 63) / 64;
   mi_tile_cfg best = t[0].cfg;
   double least = 1e30;
@@ -257,7 +261,13 @@ mi_tile_cfg pick(int M, int N, int K, bool bt) {
       const long long blocks = (tiles * parts + cus - 1) / cus, rounds = (blocks + e.per_cu - 1) / e.per_cu;
       const double in_line = (double)blocks * e.shared * each, alone = (double)rounds * e.alone * each;
       double us = (in_line > alone ? in_line : alone) + (double)rounds * e.ends;
-      if (us < mem) us = mem;
+      if (streamed) {
+        const double cold = (double)rounds * ((double)each * e.cold + e.ends), blocks_us = us > cold ? us : cold;
+        const double mem = bytes / (e.stream * 1e6);
+        us = std::cbrt(blocks_us * blocks_us * blocks_us + mem * mem * mem);
+      } else if (us < bytes / 5.4e6) {
+        us = bytes / 5.4e6;
+      }
       if (parts > 1) us += 3.0 + (double)parts * M * N * 2e-6;
       if (us < least) {
         least = us;

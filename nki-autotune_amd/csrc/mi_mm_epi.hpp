@@ -24,8 +24,9 @@
 // TFLOP/s at 8192^3: that size with bias, gelu_tanh and the kept
 // pre-activation 793 us, 1390 TFLOP/s (MFMAs busy 74 % of the time, the rest
 // mostly waits at the barriers); 1000 x 5000 x 4104 with a residual 57 us,
-// where 80 blocks of 256x256 or 320 of 128x128 leave units idle; 16 x 28672 x
-// 8192 with silu 88 us, 5.3 TB/s of weight.
+// where 160 blocks of 128x256 leave 96 units idle (blocks of 192x128 fill 240
+// and take 61: four waves alone on a unit run its MFMAs slower); 16 x 28672 x
+// 8192 with silu 78 us, 6.0 TB/s.
 #pragma once
 #include <type_traits>
 
