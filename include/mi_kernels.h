@@ -324,7 +324,8 @@ int mi_matmul_epilogue_backward_bf16(const mi_epilogue_grad_args* args, void* wo
  * (bf16 or fp32, contiguous) after `steps` steps, bf16: X = grad /
  * (||grad||_F + eps), turned where m > n; then steps times A = X X^T, X =
  * a X + (b A + c A A) X.  The iterates are held in 16 bits of mantissa (two
- * bf16) and the products accumulate in fp32.  Any sizes; a matrix's planes
+ * bf16) and the products accumulate in fp32, in an order fixed by the sizes
+ * and the batch.  Any sizes; a matrix's planes
  * (4 bytes an element, the longer side rounded up to 32, 512 rows more than
  * the shorter has) under 4 GiB, no side over 2^20, at most 65535 matrices
  * (MI_E_RANGE). */

@@ -22,7 +22,9 @@
 // columns are products with 0.
 //
 // A and A A are symmetric: only blocks on and above the diagonal are
-// computed, and each one above is stored twice, the second time turned.
+// computed, and each one above is stored twice, the second time turned.  X X^T
+// of few rows of a long X has few blocks of many K tiles: it is split over K
+// (ns_split_kernel).
 #pragma once
 #include "mi_mm_epi.hpp"
 
@@ -309,6 +311,34 @@ __global__ __launch_bounds__(WAVES * 64) void ns_product_kernel(const NsMM p, co
   NsRows rows;
   rows.init(o, z, tm * BM, BM, tn * BN, SYM && tm != tn ? BN : 0);
   epi_rows<C::TM, C::TN, C::TURN_ROW, SYM>(acc, smem, wave, lane, row0, col0, rows, tm * BM);
+}
+
+// Parts of A = X X^T over ranges of K tiles: fp32 products of the blocks on
+// and above the diagonal to ws[matrix][part][M][N]; ns_sum_kernel adds them.
+// For few rows of a long X, whose blocks would leave most units idle.
+template <int BM, int WAVES, int STAGES>
+__global__ __launch_bounds__(WAVES * 64) void ns_split_kernel(const NsMM p, float* __restrict__ ws, int parts) {
+  using C = EpiCfg<BM, BM, 64, WAVES, STAGES>;
+  using G = typename C::G;
+  __shared__ __attribute__((aligned(1024))) char smem[C::LDS_BYTES];
+  const int w = (int)blockIdx.x / parts, part = (int)blockIdx.x - w * parts;
+  int tn = (int)((__builtin_sqrtf(8.0f * (float)w + 1.0f) - 1.0f) * 0.5f);
+  while (tn * (tn + 1) / 2 > w) --tn;
+  while ((tn + 1) * (tn + 2) / 2 <= w) ++tn;
+  const int tm = __builtin_amdgcn_readfirstlane(w - tn * (tn + 1) / 2);
+  tn = __builtin_amdgcn_readfirstlane(tn);
+  const int kts = p.kw / 32, each = (kts + parts - 1) / parts, kt0 = part * each;
+  const long long z = blockIdx.y;
+  NsMM q = p;
+  q.kw = (kts - kt0 < each ? kts - kt0 : each) * 32;
+  q.a_bytes -= (uint32_t)kt0 * 128u;
+  q.b_bytes -= (uint32_t)kt0 * 128u;
+  f32x4_t acc[C::TM][C::TN];
+  ns_main<BM, BM, WAVES, STAGES, true>(q, p.a + z * p.batch_a + kt0 * 64, p.b + z * p.batch_b + kt0 * 64, smem, tm, tn, acc);
+  const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  EpiPart f;
+  f.init(ws + ((size_t)z * (size_t)parts + (size_t)part) * (size_t)p.M * (size_t)p.N, p.M, p.N, tm * BM, BM);
+  epi_rows<C::TM, C::TN, C::TURN_ROW>(acc, smem, wave, lane, (wave / G::WN) * G::WTM, tn * BM + (wave % G::WN) * G::WTN, f);
 }
 
 }  // namespace mi

@@ -123,6 +123,60 @@ __global__ __launch_bounds__(256) void ns_init_kernel(const NsInit p) {
   }
 }
 
+// A [s][2 * sp] = the sum of ns_split_kernel's parts, in their order: a block
+// of 64 x 64 on or above the diagonal, and the same turned below it.
+__global__ __launch_bounds__(256) void ns_sum_kernel(const float* __restrict__ ws, uint16_t* __restrict__ a, int parts,
+                                                     int s, int sp) {
+  __shared__ float tile[64][65];
+  const int tid = (int)threadIdx.x, w = (int)blockIdx.x;
+  int tn = (int)((__builtin_sqrtf(8.0f * (float)w + 1.0f) - 1.0f) * 0.5f);
+  while (tn * (tn + 1) / 2 > w) --tn;
+  while ((tn + 1) * (tn + 2) / 2 <= w) ++tn;
+  const int m0 = (w - tn * (tn + 1) / 2) * 64, n0 = tn * 64;
+  const size_t stride = (size_t)s * (size_t)sp;
+  const float* part = ws + (size_t)blockIdx.y * (size_t)parts * stride;
+  uint16_t* out = a + (size_t)blockIdx.y * 2 * stride;
+  const auto store = [&](int row, int col, const float(&v)[8]) __attribute__((always_inline)) {
+    float t[8];
+    const mi::u32x4_t hi = mi::pack8(v);
+    mi::unpack8(hi, t);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) t[k] = v[k] - t[k];
+    uint16_t* at = out + (size_t)row * (size_t)(2 * sp) + mi::ns_at(col);
+    *(mi::u32x4_t*)at = hi;
+    *(mi::u32x4_t*)(at + 32) = mi::pack8(t);
+  };
+  const int c = tid % 8 * 8;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int r = tid / 8 + 32 * j;
+    float v[8] = {};
+    if (m0 + r < s && n0 + c < sp) {
+      const float* at = part + (size_t)(m0 + r) * (size_t)sp + n0 + c;
+      const mi::f32x4_t lo = mi::sum_in_order<0>((const mi::f32x4_t*)at, stride, parts);
+      const mi::f32x4_t hi = mi::sum_in_order<0>((const mi::f32x4_t*)(at + 4), stride, parts);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        v[k] = lo[k];
+        v[4 + k] = hi[k];
+      }
+      store(m0 + r, n0 + c, v);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) tile[r][c + k] = v[k];
+  }
+  if (m0 == n0) return;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int r = tid / 8 + 32 * j;
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = tile[c + k][r];
+    if (n0 + r < s && m0 + c < sp) store(n0 + r, m0 + c, v);
+  }
+}
+
 // out [m][n] from the hi values of X [s][2 * lp], turned back where G was: hi
 // is the value rounded to bf16.
 __global__ __launch_bounds__(256) void ns_last_kernel(const uint16_t* __restrict__ x, uint16_t* __restrict__ out, int m,
@@ -172,9 +226,11 @@ size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 struct Plan {
   int s, l, sp, lp, parts;
+  int split;  // parts of X X^T (1: none)
   bool turn;
-  size_t x0, x1, a, b, part, bytes;
+  size_t x1, a, b, part, gram, bytes;
 };
+int gram_parts(int s, int sp, int lp, int batch);
 int ns_plan(const mi_newton_schulz_args* p, Plan* q) {
   if (p->batch < 0 || p->m < 0 || p->n < 0) return fail(MI_E_ARGS, "negative size batch=%d m=%d n=%d", p->batch, p->m, p->n);
   if (p->steps < 0) return fail(MI_E_ARGS, "steps=%d negative", p->steps);
@@ -200,7 +256,9 @@ int ns_plan(const mi_newton_schulz_args* p, Plan* q) {
   q->a = 2 * x;
   q->b = q->a + a;
   q->part = q->b + a;
-  q->bytes = q->part + up256((size_t)p->batch * q->parts * 8);
+  q->gram = q->part + up256((size_t)p->batch * q->parts * 8);
+  q->split = p->steps > 0 ? gram_parts(q->s, q->sp, q->lp, p->batch) : 1;
+  q->bytes = q->gram + (q->split > 1 ? up256((size_t)p->batch * q->split * q->s * q->sp * 4) : 0);
   return MI_OK;
 }
 
@@ -242,10 +300,46 @@ int fastest(const NsBlock (&b)[N], const NsMM& p, bool sym, int batch) {
   }
   return best;
 }
+constexpr NsBlock kSymmetric[] = {
+    {64, 2, 0.205, 0.235, 3.875}, {128, 1, 0.538, 0.467, 6.619}, {192, 1, 0.949, 1.036, 12.722}};
+// How many parts X X^T is split into: as many as the least estimated time
+// takes, a part of at least 4 K tiles; parts cost a second launch and their
+// products written and read.  Five steps of 640 x 6000 take 227 us in 4 parts
+// and 319 unsplit, 64 x 2048 77 in 8 and 109, 2001 x 777 185 in 2 and 195; of
+// 1024 x 4096, whose blocks take more than half the units, 331 in 4 and 328,
+// 1000 x 3000 303 and 287.
+int gram_parts(int s, int sp, int lp, int batch) {
+  const int cus = mi::capi::device_cus(), kts = lp / 32;
+  double least = 1e30;
+  for (const NsBlock& b : kSymmetric) {
+    const long long t = (sp + b.bm - 1) / b.bm;
+    const double us = estimate(b, batch * (t * (t + 1) / 2), kts, cus);
+    if (us < least) least = us;
+  }
+  int best = 1;
+  const long long t = (sp + 63) / 64, tri = t * (t + 1) / 2;
+  for (const int parts : {2, 4, 8}) {
+    const int each = (kts + parts - 1) / parts;
+    const double bytes = (double)batch * parts * s * sp * 4.0;
+    if (each < 4 || (parts - 1) * each >= kts || bytes > (double)mi::capi::kMaxWorkspace) break;
+    const double us = estimate(kSymmetric[0], batch * tri * parts, each, cus) + 5.0 + bytes / 2.5e6;
+    if (us < least) {
+      least = us;
+      best = parts;
+    }
+  }
+  return best;
+}
+int split_gram(const NsMM& p, uint16_t* a, float* ws, int parts, int batch, hipStream_t s) {
+  const unsigned t = (unsigned)((p.N + 63) / 64), tri = t * (t + 1) / 2;
+  mi::ns_split_kernel<64, 4, 4><<<dim3(tri * (unsigned)parts, (unsigned)batch), dim3(256), 0, s>>>(p, ws, parts);
+  const int rc = launched("parts of a Newton-Schulz product");
+  if (rc != MI_OK) return rc;
+  ns_sum_kernel<<<dim3(tri, (unsigned)batch), dim3(256), 0, s>>>(ws, a, parts, p.M, p.N);
+  return launched("sum of the parts");
+}
 int symmetric(const NsMM& p, const NsOut& o, int batch, hipStream_t s) {
-  static constexpr NsBlock blocks[] = {
-      {64, 2, 0.205, 0.235, 3.875}, {128, 1, 0.538, 0.467, 6.619}, {192, 1, 0.949, 1.036, 12.722}};
-  switch (fastest(blocks, p, true, batch)) {
+  switch (fastest(kSymmetric, p, true, batch)) {
     case 64: return product<64, 64, 4, 4, true, true>(p, o, batch, s);
     case 128: return product<128, 128, 4, 4, true, true>(p, o, batch, s);
     default: return product<192, 192, 4, 3, true, true>(p, o, batch, s);
@@ -311,7 +405,8 @@ int mi_newton_schulz(const mi_newton_schulz_args* args, void* workspace, unsigne
   for (int k = 0; k < args->steps; ++k) {
     const NsMM gram = {x, x, xb, xb, s, sp, lp, lp, lp, xz, xz};
     const NsOut to_a = {nullptr, A, nullptr, s, sp, 1.0f, 0.0f, 0, az, 0};
-    if ((rc = symmetric(gram, to_a, batch, st)) != MI_OK) return rc;
+    rc = q.split > 1 ? split_gram(gram, A, (float*)(ws + q.gram), q.split, batch, st) : symmetric(gram, to_a, batch, st);
+    if (rc != MI_OK) return rc;
     const NsMM square = {A, A, ab, ab, s, sp, sp, sp, sp, az, az};
     const NsOut to_b = {A, B, nullptr, s, sp, args->c, args->b, az, az, 0};
     if ((rc = symmetric(square, to_b, batch, st)) != MI_OK) return rc;

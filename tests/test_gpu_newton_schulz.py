@@ -8,7 +8,7 @@ from block_oracle import newton_schulz as ns64
 pytestmark = pytest.mark.gpu
 
 SHAPES = [(1, 1), (1, 9), (9, 1), (2, 3), (31, 33), (64, 64), (65, 63), (40, 300), (300, 40), (128, 513), (200, 200),
-          (257, 129), (777, 100), (1, 5000), (512, 1024)]
+          (257, 129), (777, 100), (1, 5000), (512, 1024), (100, 2100), (3001, 129), (640, 4000)]
 
 
 def _grad(shape, dtype, gpu, seed=0, scale=1e-3):
@@ -53,7 +53,7 @@ def test_shapes(gpu, m, n, dtype):
     _check(out, grad)
 
 
-@pytest.mark.parametrize("shape", [(3, 40, 72), (5, 130, 64), (2, 512, 256), (4, 1, 7), (2, 300, 1000)])
+@pytest.mark.parametrize("shape", [(3, 40, 72), (5, 130, 64), (2, 512, 256), (4, 1, 7), (2, 300, 1000), (3, 300, 2000)])
 def test_a_batch_is_its_matrices(gpu, shape):
     import torch
 
@@ -142,12 +142,13 @@ def test_only_the_output_is_written(gpu):
         assert (big[:512 + off] == 7).all() and (big[512 + off + m * n:] == 7).all()
 
 
-def test_same_bits_on_streams_and_in_graphs(gpu):
+@pytest.mark.parametrize("shape", [(2, 130, 200), (2, 100, 3000)])
+def test_same_bits_on_streams_and_in_graphs(gpu, shape):
     import torch
 
     import kernel_library as kl
 
-    grad = _grad((2, 130, 200), "float32", gpu)
+    grad = _grad(shape, "float32", gpu)
     want = kl.newton_schulz(grad)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -162,7 +163,7 @@ def test_same_bits_on_streams_and_in_graphs(gpu):
             out = kl.newton_schulz(grad)
         graphs.append((graph, out))
     for k in range(3):
-        grad.copy_(_grad((2, 130, 200), "float32", gpu, seed=k + 1))
+        grad.copy_(_grad(shape, "float32", gpu, seed=k + 1))
         want = kl.newton_schulz(grad)
         torch.cuda.synchronize()
         for graph, out in graphs:

@@ -144,3 +144,48 @@ def test_negated_views_are_refused(gpu):
     assert v.is_neg()
     with pytest.raises(ValueError, match="negated"):
         kl.layer_norm(v)
+
+
+def test_two_threads_at_once(gpu):
+    """Calls from two threads, each on a stream of its own: workspaces, errors and answers stay apart."""
+    import threading
+
+    import torch
+
+    import kernel_library as kl
+
+    bf = torch.bfloat16
+    failed = []
+
+    def work(seed):
+        try:
+            g = torch.Generator().manual_seed(seed)
+            M, N, K = (40, 520, 2048) if seed else (70, 131, 333)
+            lhs, rhs, r = (torch.randn(*s, generator=g).to(bf).to(gpu) for s in ((M, K), (K, N), (M, N)))
+            grad = torch.randn(100 + seed, 2100, generator=g).to(bf).to(gpu)
+            stream = torch.cuda.Stream()
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                def step():
+                    y, mean, rstd = kl.layer_norm(r, stats=True)
+                    out = kl.matmul_epilogue(lhs, rhs, None, "silu", y)
+                    return (out, *kl.matmul_epilogue_backward(r, lhs, rhs, "silu", out)[:2],
+                            kl.layer_norm_backward(out, r, mean, rstd)[0], kl.newton_schulz(grad))
+
+                want = step()
+                for _ in range(20):
+                    with pytest.raises(ValueError, match="contraction mismatch"):
+                        kl.matmul_epilogue(lhs, rhs[1:])
+                    got = step()
+                    stream.synchronize()
+                    assert all(bool((a == b).all()) for a, b in zip(got, want))
+        except BaseException as e:  # noqa: BLE001 -- reported by the main thread
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert not failed, failed
+    assert not any(t.is_alive() for t in threads)
