@@ -291,7 +291,8 @@ int mi_layer_norm_backward(const mi_layer_norm_grad_args* args, void* workspace,
  * cfg: block_m, block_n, block_k, waves, lds_stages and variant (1: rhs read
  * non-temporally, for few rows) of one of mi_epilogue_config's, split_k
  * 1..16 (every part at least one K tile; 1 where N > 2^20) and group_m (0:
- * 8); NULL: the library's choice for the shape. */
+ * 8; all tile rows where there are no more); NULL: the library's choice for
+ * the shape. */
 enum { MI_ACT_NONE = 0, MI_ACT_RELU = 1, MI_ACT_GELU = 2, MI_ACT_GELU_TANH = 3, MI_ACT_SILU = 4 };
 typedef struct {
   const void *lhs, *rhs, *bias, *residual;

@@ -315,7 +315,7 @@ int plan(const uint16_t* a, int lda, const uint16_t* b, int ldb, long long b_row
   if (out->ws_bytes > mi::capi::kMaxWorkspace)
     return fail(MI_E_RANGE, "split-K workspace of %zu bytes exceeds %llu", out->ws_bytes, mi::capi::kMaxWorkspace);
   out->mm = EpiMM{a, b, (uint32_t)((size_t)M * lda * 2), (uint32_t)((size_t)b_rows * ldb * 2), M, N, K, lda, ldb,
-                  c.group_m > 0 ? c.group_m : 8, c.split_k};
+                  mi::capi::raster_group(c.group_m, M, c.block_m), c.split_k};
   return MI_OK;
 }
 // The blocks of the products of operands as they are: 32 x 128, or 64 x 64

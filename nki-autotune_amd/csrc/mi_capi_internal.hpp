@@ -21,6 +21,15 @@ inline unsigned long long f32_kw_span(int cols, int K, int block) {
   return (rows * (unsigned long long)cols + (unsigned long long)block) * 4ull;
 }
 
+// Tile rows of a raster group: a config's group_m (0: 8), at most those that M
+// has.  More are the same one group of all, but the kernels multiply the group
+// by the tile columns in 32 bits, where a group of 2^30 wraps to a width of 0
+// or less and tiles far outside the output.
+inline int raster_group(int group_m, int M, int block_m) {
+  const int rows = (int)(((long long)M + block_m - 1) / block_m), group = group_m > 0 ? group_m : 8;
+  return group < rows ? group : rows;
+}
+
 // Records the message of a failure for mi_last_error on this thread and
 // returns `code`.
 int fail(int code, const char* fmt, ...);
