@@ -92,7 +92,8 @@ enum {
  *                               keeps at most 256 MiB of freed workspace
  *                               cached per device; mi_release_workspace
  *                               returns all of it.
- *   group_m                   : L2 raster group height in tiles (0 = default 8)
+ *   group_m                   : L2 raster group height in tiles (0 = default
+ *                               8; all tile rows where there are no more)
  *   variant                   : kernel-specific pipeline (every variant computes
  *                               the same function):
  *     matmul         0 plain double buffer; 1 software-pipelined LDS-direct

@@ -333,7 +333,7 @@ int resolve(int kernel_id, const mi_tile_cfg* cfg_in, const mi::MiArgs& a, mi_ti
 int launch(const mi::MiEntry* e, const mi_tile_cfg& cfg, const mi::MiArgs& args_in, char* ws, bool ws_zeroed,
            void* stream) {
   mi::MiArgs a = args_in;
-  a.group_m = cfg.group_m > 0 ? cfg.group_m : 8;
+  a.group_m = mi::capi::raster_group(cfg.group_m, a.M, cfg.block_m);
   a.parts = cfg.split_k;
   a.ws = ws;
   a.ws_zeroed = ws_zeroed;
