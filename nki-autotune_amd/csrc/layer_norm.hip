@@ -128,7 +128,7 @@ void bwd_run(const LnBwd& p, const BwdPlan& b, hipStream_t s) {
 
 int check_common(long long rows, int D, long long ldx, int dtype) {
   if (rows < 0 || D <= 0) return fail(MI_E_ARGS, "bad size rows=%lld D=%d (D must be positive)", rows, D);
-  if (D > 1 << 28) return fail(MI_E_RANGE, "D=%d over %d", D, 1 << 28);  // one launch adds up the parameters' gradients
+  if (D > 1 << 28) return fail(MI_E_RANGE, "D=%d over %d", D, 1 << 28);  // indexes run a block's stride past D in 32 bits
   if (ldx < 0) return fail(MI_E_ARGS, "negative row stride %lld", ldx);
   if (dtype != MI_DTYPE_BF16 && dtype != MI_DTYPE_F16 && dtype != MI_DTYPE_F32)
     return fail(MI_E_ARGS, "unknown dtype %d", dtype);
@@ -215,7 +215,7 @@ int mi_layer_norm_backward(const mi_layer_norm_grad_args* a, void* workspace, un
   const int lrc = launched("layer norm gradient");
   if (lrc != MI_OK || !need) return lrc;
   const ColumnSum c = {(const float*)workspace, {a->dweight, a->dbias}, b.blocks, a->D};
-  const dim3 grid((unsigned)((a->D + 63) / 64), 2);
+  const dim3 grid(mi::column_sum_blocks(a->D), 2);
   if (f32 || a->params_f32) mi::column_sum_kernel<float><<<grid, dim3(1024), 0, s>>>(c);
   else if (a->dtype == MI_DTYPE_BF16) mi::column_sum_kernel<Bf16><<<grid, dim3(1024), 0, s>>>(c);
   else mi::column_sum_kernel<Fp16><<<grid, dim3(1024), 0, s>>>(c);

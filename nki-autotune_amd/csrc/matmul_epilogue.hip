@@ -469,7 +469,7 @@ int bwd_plan(const mi_epilogue_grad_args* a, char* ws, Bwd* b) {
     return at;
   };
   if (a->dbias) {
-    if (N > 1 << 28) return fail(MI_E_RANGE, "dbias of %d columns, over %d", N, 1 << 28);  // one launch adds them up
+    if (N > 1 << 28) return fail(MI_E_RANGE, "dbias of %d columns, over %d", N, 1 << 28);  // the same limit as layer norm's
     const int xb = (up8(N) + 511) / 512;
     const int rows4 = (a->M + 3) / 4, want = 2048 / xb;
     b->chunks = want < 1 ? 1 : want > 256 ? 256 : want;
@@ -662,7 +662,7 @@ int mi_matmul_epilogue_backward_bf16(const mi_epilogue_grad_args* a, void* works
     if ((rc = launched("activation gradient")) != MI_OK) return rc;
     if (a->dbias) {
       const mi::ColumnSum c = {g.part, {a->dbias, nullptr}, chunks, N};
-      const dim3 grid((unsigned)((N + 63) / 64), 1);
+      const dim3 grid(mi::column_sum_blocks(N), 1);
       if (a->bias_f32) mi::column_sum_kernel<float><<<grid, dim3(1024), 0, s>>>(c);
       else mi::column_sum_kernel<mi::Bf16><<<grid, dim3(1024), 0, s>>>(c);
       if ((rc = launched("bias gradient")) != MI_OK) return rc;
