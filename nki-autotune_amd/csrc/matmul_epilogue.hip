@@ -215,6 +215,9 @@ unsigned blocks_for(long long items) {
 // and not split.
 constexpr int kWide = 1 << 20;
 
+// A launch holds fewer than 2^32 threads.
+bool launches(long long blocks, int threads) { return blocks * threads < 1ll << 32; }
+
 int up8(int v) { return (v + 7) / 8 * 8; }
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 bool at16(const void* p) { return (uintptr_t)p % 16 == 0; }
@@ -252,6 +255,7 @@ mi_tile_cfg pick(int M, int N, int K, bool bt) {
     const EpiEntry& e = t[i];
     const long long tiles =
         (long long)((M + e.cfg.block_m - 1) / e.cfg.block_m) * ((N + e.cfg.block_n - 1) / e.cfg.block_n);
+    if (!launches(tiles, e.cfg.waves * 64)) continue;  // small blocks of an output past 128 GB
     for (const int parts : {1, 2, 3, 4, 6, 8, 12, 16}) {
       const int each = (kt + parts - 1) / parts;
       // Parts of at least three K tiles, none empty, in at most four blocks a unit.
@@ -308,6 +312,9 @@ int plan(const uint16_t* a, int lda, const uint16_t* b, int ldb, long long b_row
                                        : ((unsigned long long)K + c.block_k) * ldb * 2ull + 2ull * c.block_n;
   if (a_span > kMaxOffset || b_span > kMaxOffset)
     return fail(MI_E_RANGE, "operand spans exceed 32-bit buffer offsets (%llu, %llu bytes)", a_span, b_span);
+  const long long tiles = ((long long)M + c.block_m - 1) / c.block_m * (((long long)N + c.block_n - 1) / c.block_n);
+  if (!launches(tiles * c.split_k, c.waves * 64))
+    return fail(MI_E_RANGE, "%lld blocks of %d threads are over a launch's 2^32 threads", tiles * c.split_k, c.waves * 64);
   out->any = false;
   out->e = e;
   out->ldw = up8(N);
@@ -365,7 +372,10 @@ int run(const Product& p, const EpiOut& o, float* ws, hipStream_t s) {
 // 153 with copies (198 MB: 5 TB/s and 1.3), 200 x 4001 x 4001 37 and 38.  Past
 // that the padded kernels' larger blocks win: 500 x 2001 x 3001 31 and 25 us,
 // 1000 x 5001 x 4001 110 and 78.
-bool better_as_is(int M, int N, int K, bool bt) { return M <= 256 && K >= 8 && (bt || N >= 8); }
+bool better_as_is(int M, int N, int K, bool bt) {
+  if (M > 256 || K < 8 || (!bt && N < 8)) return false;
+  return launches((long long)((M + any_bm(M) - 1) / any_bm(M)) * ((N + any_bn(M) - 1) / any_bn(M)), 256);
+}
 
 // An operand that needs padded rows: its copy's place in the workspace.
 struct Padded {
