@@ -258,7 +258,11 @@ mi_tile_cfg pick(int M, int N, int K, bool bt) {
     if (!launches(tiles, e.cfg.waves * 64)) continue;  // small blocks of an output past 128 GB
     for (const int parts : {1, 2, 3, 4, 6, 8, 12, 16}) {
       const int each = (kt + parts - 1) / parts;
-      // Parts of at least three K tiles, none empty, in at most four blocks a unit.
+      // Parts of at least three K tiles, none empty, in at most four blocks a
+      // unit.  The first count that does not fit ends the search: at 61 to 64,
+      // 76, 77, 109, 110 and 121 K tiles 12 parts leave one empty and 16 do
+      // not, but those take 1.07 times what is chosen so (40 shapes of 1 to
+      // 512 rows, 0.98 to 1.19).
       if (parts > 1 && (N > kWide || kt / parts < 3 || (parts - 1) * each >= kt || tiles * parts > 4ll * cus ||
                         (double)parts * M * N * 4.0 > (double)mi::capi::kMaxWorkspace))
         break;
