@@ -64,7 +64,7 @@ struct NsInit {
 template <class T>
 __global__ __launch_bounds__(256) void ns_init_kernel(const NsInit p) {
   __shared__ float tile[64][65];
-  __shared__ float scale_lds;
+  __shared__ double scale_lds;
   const int tid = (int)threadIdx.x, z = (int)blockIdx.z;
   const T* g = (const T*)p.g + (size_t)z * (size_t)p.m * (size_t)p.n;
   const int r0 = (int)blockIdx.y * 64, c0 = (int)blockIdx.x * 64;  // of X
@@ -93,7 +93,7 @@ __global__ __launch_bounds__(256) void ns_init_kernel(const NsInit p) {
       t[i] = tid + 64 * i < p.parts ? p.part[(size_t)z * p.parts + tid + 64 * i] : 0.0;
     double sum = (t[0] + t[1]) + (t[2] + t[3]);
     for (int k = 32; k > 0; k >>= 1) sum += __shfl_xor(sum, k);
-    if (tid == 0) scale_lds = (float)(1.0 / (__builtin_sqrt(sum) + (double)p.eps));
+    if (tid == 0) scale_lds = 1.0 / (__builtin_sqrt(sum) + (double)p.eps);
   }
 #pragma unroll
   for (int j = 0; j < 2; ++j)
@@ -105,14 +105,18 @@ __global__ __launch_bounds__(256) void ns_init_kernel(const NsInit p) {
       else tile[a][b] = v;
     }
   __syncthreads();
-  const float scale = scale_lds;
+  // A scale that fp32 holds in full, or, of a norm under 2^-128 or past 2^126,
+  // one that it does not, in 64 bits.
+  const double exact = scale_lds;
+  const float scale = (float)exact;
+  const bool held = scale >= 0x1p-126f && scale <= 0x1.fffffep127f;
   uint16_t* x = p.x + (size_t)z * (size_t)p.s * (size_t)(2 * p.lp);
   for (int i = tid; i < 64 * 8; i += 256) {
     const int r = i / 8, c = (i % 8) * 8;
     if (r0 + r >= p.s || c0 + c >= p.lp) continue;
     float v[8], t[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = tile[r][c + k] * scale;
+    for (int k = 0; k < 8; ++k) v[k] = held ? tile[r][c + k] * scale : (float)((double)tile[r][c + k] * exact);
     const mi::u32x4_t hi = mi::pack8(v);
     mi::unpack8(hi, t);
 #pragma unroll

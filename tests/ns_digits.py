@@ -41,7 +41,7 @@ def emulated(grad: torch.Tensor, steps: int = 5, eps: float = 1e-7, a=1, b=1, x=
     p, q, r = COEFFICIENTS
     turn = grad.shape[0] > grad.shape[1]
     v = grad.float().t().contiguous() if turn else grad.float()
-    v = v * float(1 / (torch.linalg.norm(v.double()) + eps))
+    v = (v.double() / (torch.linalg.norm(v.double()) + eps)).float()
     X = _halves(v)
     for _ in range(steps):
         A = _halves(_product(X, tuple(t.t().contiguous() for t in X), gram), a)

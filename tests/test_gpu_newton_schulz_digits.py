@@ -41,3 +41,22 @@ def test_steps(gpu, steps):
         d, most = distance(kl.newton_schulz(grad, steps=steps), grad, steps), allowed(grad, steps)
         print(f"newton_schulz {m}x{n}, {steps} steps: {d:.2e} of {most:.2e}", flush=True)
         assert d <= most
+
+
+def test_norms_whose_reciprocal_leaves_fp32(gpu):
+    """fp32 gradients near either end of its range, without an eps: 1 / norm is past the largest number, or has lost
+    digits under the smallest normal one."""
+    import torch
+
+    import kernel_library as kl
+
+    for m, n in ((70, 100), (129, 64)):
+        for scale in (1e-41, 3e-43, 5e37):
+            grad = _grad((m, n), "float32", gpu, scale=1.0)
+            grad = (grad.double() / float(grad.abs().max()) * scale * 5).float()
+            assert torch.isfinite(grad).all() and float(grad.abs().max()) > 0
+            d, most = distance(kl.newton_schulz(grad, eps=0.0), grad, eps=0.0), allowed(grad * 1.0, eps=0.0)
+            print(f"newton_schulz {m}x{n} {scale}: {d:.2e} of {most:.2e}", flush=True)
+            assert d <= most
+    zero = torch.zeros(40, 50, device=gpu)
+    assert (kl.newton_schulz(zero, eps=1e-42) == 0).all()
