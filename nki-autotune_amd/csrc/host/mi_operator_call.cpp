@@ -9,8 +9,11 @@
 // bind_operators() was not told of.  The Python body then runs, checks
 // everything and raises what is to be raised.  Nothing is kept between calls
 // but the entry points.
+#include <c10/core/GradMode.h>
+
 #include <climits>
 #include <cstdlib>
+#include <initializer_list>
 #include <string>
 #include <vector>
 
@@ -18,6 +21,11 @@
 #include "mi_torch_plain.hpp"
 
 extern PyMethodDef kOperatorMethods[];
+
+// The same words as the Python bodies' (_operands.warn_detached).
+#define MI_DETACHED                                                                                          \
+  "%s records nothing for autograd, and an operand requires a gradient: it will not reach it through this " \
+  "result. Call %s under torch.no_grad() and take the gradients from the operator's own call."
 
 namespace {
 
@@ -76,6 +84,15 @@ PyObject* raise(int rc, const char* what) {
     PyErr_SetString(PyExc_RuntimeError, what);
   }
   return nullptr;
+}
+
+// Warns where autograd records and an operand requires a gradient: the result
+// will not.  False where the warning is an error.
+bool warn_detached(const char* what, std::initializer_list<const at::Tensor*> operands) {
+  if (!c10::GradMode::is_enabled()) return true;
+  for (const at::Tensor* t : operands)
+    if (t && t->requires_grad()) return PyErr_WarnFormat(PyExc_UserWarning, 2, MI_DETACHED, what, what) == 0;
+  return true;
 }
 
 // fn(stream) without the GIL; fn reads nothing shared.
@@ -167,7 +184,7 @@ PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
       MI_OR_PYTHON(given->scalar_type() == x->scalar_type() && given->sizes() == x->sizes() && disjoint(*given, *x) &&
                    (!w || disjoint(*given, *w)) && (!b || disjoint(*given, *b)));
     const int stats = PyObject_IsTrue(args[5]);
-    if (stats < 0) return nullptr;
+    if (stats < 0 || !warn_detached("layer_norm", {x, w, b})) return nullptr;
     const c10::OptionalDeviceGuard guard(dev);
     at::Tensor out = given ? *given : like(*x), mean, rstd;
     if (stats) {
@@ -271,6 +288,7 @@ PyObject* matmul_epilogue(PyObject*, PyObject* const* args, Py_ssize_t n) {
       for (const at::Tensor* i : {lhs, rhs, bias, res}) MI_OR_PYTHON(!i || disjoint(*o, *i));
     }
     MI_OR_PYTHON(!pre || !given || disjoint(*pre, *given));
+    if (!warn_detached("matmul_epilogue", {lhs, rhs, bias, res})) return nullptr;
     const c10::OptionalDeviceGuard guard(dev);
     at::Tensor out = given ? *given : make(*lhs, {z.M, z.N}, at::kBFloat16);
     const mi_epilogue_args a = {lhs->data_ptr(), rhs->data_ptr(), ptr(bias), ptr(res), out.data_ptr(), ptr(pre), (int)z.M,
@@ -340,6 +358,7 @@ PyObject* newton_schulz(PyObject*, PyObject* const* args, Py_ssize_t n) {
                  k <= INT_MAX);
     if (given)
       MI_OR_PYTHON(given->scalar_type() == at::kBFloat16 && given->sizes() == g->sizes() && disjoint(*given, *g));
+    if (!warn_detached("newton_schulz", {g})) return nullptr;
     const c10::OptionalDeviceGuard guard(g->device());
     at::Tensor out = given ? *given : make(*g, g->sizes(), at::kBFloat16);
     const mi_newton_schulz_args a = {g->data_ptr(), out.data_ptr(), (int)batch, (int)m, (int)k, (int)steps, dtype,

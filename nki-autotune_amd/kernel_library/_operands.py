@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import warnings
 from collections.abc import Callable, Container
 
 import torch
@@ -55,6 +56,15 @@ def no_overlap(name: str, out: torch.Tensor, **others: torch.Tensor | None) -> N
         t0, t1 = _span(t)
         if t0 < o1 and o0 < t1:
             raise ValueError(f"{name} overlaps {other}: an output must not alias another operand")
+
+
+def warn_detached(what: str, *operands: torch.Tensor | None) -> None:
+    """Warns (at the caller of the operator that calls this) where autograd records and an operand requires a gradient:
+    the result will not."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in operands):
+        warnings.warn(f"{what} records nothing for autograd, and an operand requires a gradient: it will not reach it "
+                      f"through this result. Call {what} under torch.no_grad() and take the gradients from the "
+                      "operator's own call.", UserWarning, stacklevel=3)
 
 
 def workspace(device: torch.device, what: str, query: Callable, *args) -> tuple[torch.Tensor | None, int]:

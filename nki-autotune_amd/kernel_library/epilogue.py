@@ -7,9 +7,9 @@
 bf16 operands and outputs, fp32 accumulation, any sizes; the bias bf16 or
 fp32.  ``rhs`` is ``[K, N]`` as in ``matmul_lhs_rhs``, or ``[N, K]`` with
 ``rhs_transposed`` (``torch.nn.Linear``'s weight).  The calls record nothing
-for torch's autograd: the gradient is a call of its own.  Every call runs HIP
-kernels (csrc/mi_mm_epi.hpp) on the current torch stream; there is no
-fallback path.
+for torch's autograd: the gradient is a call of its own, and the forward call
+warns where autograd would expect one.  Every call runs HIP kernels
+(csrc/mi_mm_epi.hpp) on the current torch stream; there is no fallback path.
 """
 
 from __future__ import annotations
@@ -19,7 +19,7 @@ import ctypes
 import torch
 
 from kernel_library import _lib
-from kernel_library._operands import int32, launch, no_overlap, tensor, workspace
+from kernel_library._operands import int32, launch, no_overlap, tensor, warn_detached, workspace
 from kernel_library.config import TileConfig, _torch_call
 
 _ACTIVATIONS = {None: _lib.MI_ACT_NONE, "none": _lib.MI_ACT_NONE, "relu": _lib.MI_ACT_RELU, "gelu": _lib.MI_ACT_GELU,
@@ -111,6 +111,7 @@ def matmul_epilogue(
     else:
         _matrix("out", out, M, N, lhs)
         no_overlap("out", out, lhs=lhs, rhs=rhs, bias=bias, residual=residual, pre=pre)
+    warn_detached("matmul_epilogue", lhs, rhs, bias, residual)
     args = _lib.EpilogueArgs(lhs.data_ptr(), rhs.data_ptr(), _ptr(bias), _ptr(residual), out.data_ptr(), _ptr(pre), M, N,
                              K, rhs_transposed, act, f32)
     c = None if cfg is None else ctypes.byref(cfg.to_c())

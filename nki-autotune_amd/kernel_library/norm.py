@@ -5,9 +5,10 @@
 
 bf16, fp16 or fp32 rows of any length; parameters of the rows' type or fp32;
 statistics and sums in fp32, each output rounded once.  The calls record
-nothing for torch's autograd: the gradient is a call of its own.  Every call
-runs HIP kernels (csrc/mi_norm.hpp) on the current torch stream; there is no
-fallback path.
+nothing for torch's autograd: the gradient is a call of its own, and the
+forward call warns where autograd would expect one.  Every call runs HIP
+kernels (csrc/mi_norm.hpp) on the current torch stream; there is no fallback
+path.
 """
 
 from __future__ import annotations
@@ -17,7 +18,7 @@ import ctypes
 import torch
 
 from kernel_library import _lib
-from kernel_library._operands import int32, launch, no_overlap, tensor, workspace
+from kernel_library._operands import int32, launch, no_overlap, tensor, warn_detached, workspace
 from kernel_library.config import _torch_call
 
 _DTYPES = {torch.bfloat16: _lib.MI_DTYPE_BF16, torch.float16: _lib.MI_DTYPE_F16, torch.float32: _lib.MI_DTYPE_F32}
@@ -85,6 +86,7 @@ def layer_norm(
         if out.shape != x.shape or not out.is_contiguous():
             raise ValueError(f"out must be a contiguous {x.dtype} tensor of shape {tuple(x.shape)}")
         no_overlap("out", out, x=x, weight=weight, bias=bias)
+    warn_detached("layer_norm", x, weight, bias)
     mean = rstd = None
     if stats:
         mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)

@@ -14,7 +14,7 @@ import ctypes
 import torch
 
 from kernel_library import _lib
-from kernel_library._operands import int32, launch, no_overlap, tensor, workspace
+from kernel_library._operands import int32, launch, no_overlap, tensor, warn_detached, workspace
 from kernel_library.config import _torch_call
 
 _DTYPES = {torch.bfloat16: _lib.MI_DTYPE_BF16, torch.float32: _lib.MI_DTYPE_F32}
@@ -53,6 +53,7 @@ def newton_schulz(
         if out.shape != grad.shape or not out.is_contiguous():
             raise ValueError(f"out must be a contiguous bf16 tensor of shape {tuple(grad.shape)}")
         no_overlap("out", out, grad=grad)
+    warn_detached("newton_schulz", grad)
     args = _lib.NewtonSchulzArgs(grad.data_ptr(), out.data_ptr(), batch, m, n, steps, _DTYPES[grad.dtype], *coefficients,
                                  eps)
     L = _lib.lib()
