@@ -67,11 +67,19 @@ def warn_detached(what: str, *operands: torch.Tensor | None) -> None:
                       "operator's own call.", UserWarning, stacklevel=3)
 
 
+def _on(device: torch.device, fn: Callable, *args) -> int:
+    """``fn(*args)`` with ``device`` as the current one: the library plans for, and launches on, that."""
+    if device.index == torch.cuda.current_device():
+        return fn(*args)
+    with torch.cuda.device(device):
+        return fn(*args)
+
+
 def workspace(device: torch.device, what: str, query: Callable, *args) -> tuple[torch.Tensor | None, int]:
     """The workspace that a call needs, and its bytes: from torch's allocator on the current stream, so that calls on
     several streams, and graphs, have one each."""
     need = ctypes.c_ulonglong()
-    _lib.check_rc(query(*args, ctypes.byref(need)), what)
+    _lib.check_rc(_on(device, query, *args, ctypes.byref(need)), what)
     if not need.value:
         return None, 0
     return torch.empty(need.value, dtype=torch.uint8, device=device), need.value
@@ -80,12 +88,7 @@ def workspace(device: torch.device, what: str, query: Callable, *args) -> tuple[
 def launch(device: torch.device, what: str, fn: Callable, *args) -> None:
     """``fn(*args, stream)`` on the current stream of ``device``; the native calls learn of the library that ran it."""
     stream = torch.cuda.current_stream(device).cuda_stream
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, stream)
-    else:
-        with torch.cuda.device(device):
-            rc = fn(*args, stream)
-    _lib.check_rc(rc, what)
+    _lib.check_rc(_on(device, fn, *args, stream), what)
     if not _torch_call.knows_operators():
         L = _lib.lib()
         _torch_call.bind_operators(os.environ.get("MI_KERNELS_LIB", ""),
