@@ -214,11 +214,10 @@ int mi_layer_norm_backward(const mi_layer_norm_grad_args* a, void* workspace, un
   else bwd_run<float>(p, b, s);
   const int lrc = launched("layer norm gradient");
   if (lrc != MI_OK || !need) return lrc;
-  const ColumnSum c = {(const float*)workspace, {a->dweight, a->dbias}, b.blocks, a->D};
-  const dim3 grid(mi::column_sum_blocks(a->D), 2);
-  if (f32 || a->params_f32) mi::column_sum_kernel<float><<<grid, dim3(1024), 0, s>>>(c);
-  else if (a->dtype == MI_DTYPE_BF16) mi::column_sum_kernel<Bf16><<<grid, dim3(1024), 0, s>>>(c);
-  else mi::column_sum_kernel<Fp16><<<grid, dim3(1024), 0, s>>>(c);
+  const ColumnSum c = {(const float*)workspace, {a->dweight, a->dbias}, b.blocks, a->D, 0};
+  if (f32 || a->params_f32) mi::column_sum<float>(c, 2, s);
+  else if (a->dtype == MI_DTYPE_BF16) mi::column_sum<Bf16>(c, 2, s);
+  else mi::column_sum<Fp16>(c, 2, s);
   return launched("layer norm parameter gradients");
 }
 

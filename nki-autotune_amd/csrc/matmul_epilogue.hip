@@ -675,10 +675,9 @@ int mi_matmul_epilogue_backward_bf16(const mi_epilogue_grad_args* a, void* works
     else act_grad_kernel<8><<<grid, dim3(256), 0, s>>>(g);
     if ((rc = launched("activation gradient")) != MI_OK) return rc;
     if (a->dbias) {
-      const mi::ColumnSum c = {g.part, {a->dbias, nullptr}, chunks, N};
-      const dim3 grid(mi::column_sum_blocks(N), 1);
-      if (a->bias_f32) mi::column_sum_kernel<float><<<grid, dim3(1024), 0, s>>>(c);
-      else mi::column_sum_kernel<mi::Bf16><<<grid, dim3(1024), 0, s>>>(c);
+      const mi::ColumnSum c = {g.part, {a->dbias, nullptr}, chunks, N, 0};
+      if (a->bias_f32) mi::column_sum<float>(c, 1, s);
+      else mi::column_sum<mi::Bf16>(c, 1, s);
       if ((rc = launched("bias gradient")) != MI_OK) return rc;
     }
   }

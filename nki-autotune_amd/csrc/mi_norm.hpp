@@ -510,51 +510,51 @@ static __global__ __launch_bounds__(256) void fill_zero_kernel(uint16_t* __restr
 }
 
 // out_k[d] = sum_i part[k][i][d] over i < parts, for the gridDim.y arrays k:
-// 64 columns a block at a time, its 16 waves taking turns over the parts and
-// their sums added in wave order.  Grids stay under 2^32 threads
-// (column_sum_blocks): past 2^26 columns a block takes the next 64 of its own.
+// 64 columns a block, its 16 waves taking turns over the parts and their
+// sums added in wave order.
 struct ColumnSum {
   const float* part;
   void* out[2];  // NULL: not wanted
-  int parts, D;
+  int parts, D, first;  // first: of this launch's columns
 };
-inline unsigned column_sum_blocks(int D) {
-  const int need = (D + 63) / 64, most = 1 << 20;
-  return (unsigned)(need < most ? need : most);
-}
 template <class T>
 __global__ __launch_bounds__(1024) void column_sum_kernel(const ColumnSum p) {
   __shared__ float xs[16][64];
   T* out = (T*)p.out[blockIdx.y];
   if (!out) return;
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+  const int d = p.first + (int)blockIdx.x * 64 + lane;
   const float* part = p.part + (size_t)blockIdx.y * (size_t)p.parts * (size_t)p.D;
-  for (int d0 = (int)blockIdx.x * 64;;) {
-    const int d = d0 + lane;
-    float s = 0.0f;
-    if (d < p.D) {
-      constexpr int U = 8;
-      for (int i0 = wave; i0 < p.parts; i0 += 16 * U) {
-        float v[U];
+  float s = 0.0f;
+  if (d < p.D) {
+    constexpr int U = 8;
+    for (int i0 = wave; i0 < p.parts; i0 += 16 * U) {
+      float v[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int i = i0 + 16 * u;
-          v[u] = i < p.parts ? part[(size_t)i * (size_t)p.D + d] : 0.0f;
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) s += v[u];
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + 16 * u;
+        v[u] = i < p.parts ? part[(size_t)i * (size_t)p.D + d] : 0.0f;
       }
-    }
-    xs[wave][lane] = s;
-    __syncthreads();
-    if (wave == 0 && d < p.D) {
 #pragma unroll
-      for (int w = 1; w < 16; ++w) s += xs[w][lane];
-      out[d] = from_f32<T>(s);
+      for (int u = 0; u < U; ++u) s += v[u];
     }
-    d0 += (int)gridDim.x * 64;
-    if (d0 >= p.D) break;
-    __syncthreads();  // wave 0 has read xs
+  }
+  xs[wave][lane] = s;
+  __syncthreads();
+  if (wave == 0 && d < p.D) {
+#pragma unroll
+    for (int w = 1; w < 16; ++w) s += xs[w][lane];
+    out[d] = from_f32<T>(s);
+  }
+}
+// The launches for `arrays` arrays: one, or, past 2^26 columns, one for each
+// 2^26 (a launch holds under 2^32 threads, which are 2^28 - 64 columns here).
+template <class T>
+void column_sum(ColumnSum c, unsigned arrays, hipStream_t s) {
+  constexpr int most = 1 << 26;
+  for (c.first = 0; c.first < c.D; c.first += most) {
+    const int n = c.D - c.first < most ? c.D - c.first : most;
+    column_sum_kernel<T><<<dim3((unsigned)((n + 63) / 64), arrays), dim3(1024), 0, s>>>(c);
   }
 }
 
