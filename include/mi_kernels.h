@@ -284,8 +284,10 @@ int mi_layer_norm_backward(const mi_layer_norm_grad_args* args, void* workspace,
  * [N] bf16, or fp32 (bias_f32); residual, out, pre [M,N]; all contiguous.
  * bias, residual: NULL for none.  pre: NULL, or gets lhs . rhs + bias, which
  * the gradient takes.  Any M, N, K >= 0 (K = 0: a product of 0); operands
- * under 4 GiB, sizes under 2^31 - 2^20 (MI_E_RANGE).  Operands whose rows do
- * not start on 16 bytes (K or, untransposed, N no multiple of 8, or the
+ * under 4 GiB, counting the rows that loads may run past their end (256 rows;
+ * 64 of rhs[K,N]; 1024 in rhs's gradient); sizes under 2^31 - 2^20; blocks of
+ * under 2^32 threads in all (else MI_E_RANGE).  Operands whose rows do not
+ * start on 16 bytes (K or, untransposed, N no multiple of 8, or the
  * pointer off 16) are read as they are by up to 256 rows of lhs, and by more,
  * or with a cfg, from padded copies in the workspace.
  *

@@ -125,7 +125,11 @@ __global__ __launch_bounds__(256) void epi_sum_kernel(const float* __restrict__ 
 // sums of the unrounded values over this block's rows: blockIdx.x takes 64 W
 // columns, the block's 4 waves rows 4 * blockIdx.y + wave, + 4 * gridDim.y, ...
 // A lane has W columns (8; 1 where N < 8); past the row's end the last W, of
-// which own .. W - 1 are its own.  Bound by its bytes: 22 us for 4096 x 4096
+// which own .. W - 1 are its own.  dpre is rounded because the matrix cores
+// take bf16: the products' error against float64 is then 2.35e-3, where their
+// own rounding alone leaves 1.66e-3 (1000 x 1501 x 777 and 4096^3); keeping a
+// second half as well would double both products (107 us each at 4096^3).
+// Bound by its bytes: 22 us for 4096 x 4096
 // (100 MB) on one MI355X, 4.6 TB/s.
 struct ActGrad {
   const uint16_t *dout, *pre;

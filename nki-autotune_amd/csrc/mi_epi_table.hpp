@@ -22,10 +22,18 @@
 // The last are fitted so to 19 shapes of 1 to 500 rows and rhs of 300 MB to 1
 // GB: within 1.013 on average and 1.17 at most (64 x 8192 x 28672, rhs[N,K]);
 // 4 other shapes within 1.09.
-// There non-temporal reads pay, and wide rows of rhs in one load, in whole
-// rounds of blocks: 16 x 28672 x 8192 takes 79 us with 64x256 blocks in two
-// parts and 90 with the 128x128 that the first figures alone prefer, 16 x 8192
-// x 28672 80 in eight parts and 134 with 64x64 unsplit.
+// There non-temporal reads pay, and wide rows of rhs[K,N] in one load, in
+// whole rounds of blocks: 16 x 28672 x 8192 takes 79 us with 64x256 blocks in
+// two parts and 91 with the 128x128 that the first figures alone prefer, 16 x
+// 8192 x 28672 81 with 128x128 in four parts and 134 with 64x64 unsplit.
+// rhs[N,K] goes non-temporally in 64x64: 80 us unsplit and 90 temporally, 78
+// in four parts and 128 temporally unsplit.
+//
+// A smaller rhs is taken to be in the last-level cache, as in a loop over one
+// product; where it comes from HBM, as in a decode over many layers, other
+// configs are faster (a set of weights of 1.5 GB in turn: 16 x 8192 x 8192 41
+// us and 30, 16 x 4096 x 14336 39 and 26, 32 x 10240 x 8192 59 and 36; a
+// caller's cfg reaches them).
 #define MI_EPI_CONFIGS(X)                                                     \
   X(256, 256, 64, 8, 2, 0, 0.564f, 1.304f, 11.831f, 1, 1.09f, 19.1f, 6.65f)   \
   X(256, 128, 64, 8, 3, 0, 0.720f, 0.413f, 6.953f, 1, 0.55f, 8.26f, 5.58f)    \
