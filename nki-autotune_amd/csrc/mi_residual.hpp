@@ -262,7 +262,7 @@ __global__ __launch_bounds__(B) void residual_norm_long_kernel(const RnFwd p) {
 struct RnBwd {
   const void *dy, *dhidden, *x, *hidden, *weight, *gate, *post_weight;  // dhidden: NULL for 0; x: NULL where nothing needs it
   const float *rstd, *post_rstd;  // post_rstd: NULL without a norm after the block
-  void *dx, *dresidual, *dgate;   // dx: NULL: not wanted; dgate: of a gate of one row (else NULL)
+  void *dx, *dresidual, *dgate;   // dx: NULL: not wanted; dgate: of a gate of one row each (else, or not wanted: NULL)
   float *part_w, *part_c;         // [blocks][D] partial column sums; NULL: not wanted
   float* row_dot;                 // [rows] sum_d (g * u) / D, written and read by the kernels of long rows
   long long rows, lddy, lddh, ldx, ldh;
@@ -270,6 +270,7 @@ struct RnBwd {
   int runs, per_run;              // the rows in runs of per_run, gridDim.x / runs blocks to each
   float scale;
   bool params_f32, gate_f32;
+  bool own_gates;                 // a gate of one row each: part_c's sums are those of gate * c, wanted dgate or not
 };
 
 // GROUPS rows at a time in a block of GROUPS * L threads, which stays within
@@ -390,7 +391,7 @@ __global__ __launch_bounds__(L* GROUPS) void residual_norm_bwd_kernel(const RnBw
       for (int i = 0; i < V; ++i) {
         const float t = to_f32(xv[g].v[i]) * post_rstd, s = p.scale * dh[g][i];
         const float one = s * t;
-        c[g][i] += live ? (p.dgate ? one * gt[g][i] : one) : 0.0f;
+        c[g][i] += live ? (p.own_gates ? one * gt[g][i] : one) : 0.0f;
         each[i] = one * pw[g][i];
         dh[g][i] = s * gt[g][i] * pw[g][i];  // dz from here on
         sum += split.mine(g, i, dh[g][i] * (t * inv_d));
@@ -576,9 +577,8 @@ __global__ __launch_bounds__(256) void residual_columns_kernel(const RnBwd p, in
   #pragma unroll
         for (int i = 0; i < W; ++i) dh[i] += to_f32(e.v[i]);
       }
-      // (dgate is there for a gate of one row, whose sum is that of gate * c.)
-      load_params<T>(p.dgate ? gate_at(p.gate, p.gate_f32, sizeof(T), gate_row(r, p.per_gate, p.D)) : nullptr, p.gate_f32,
-                     where, 1.0f, gt);
+      load_params<T>(p.own_gates ? gate_at(p.gate, p.gate_f32, sizeof(T), gate_row(r, p.per_gate, p.D)) : nullptr,
+                     p.gate_f32, where, 1.0f, gt);
   #pragma unroll
       for (int i = 0; i < W; ++i) c[i] += p.scale * dh[i] * (to_f32(x.v[i]) * post_rstd) * gt[0][i];
     }

@@ -55,7 +55,8 @@ Plan plan_of(const mi_residual_norm_grad_args* a) {
   p.needs_x = a->gate || a->post_rstd;
   p.sum_w = a->dweight != nullptr;
   p.sum_c = a->dpost_weight || (a->dgate && !p.own_rows);
-  p.k = mi::rn_bwd_plan(a->rows, a->D, a->dtype, p.gates > 1 && !p.own_rows && a->dgate ? p.gates : 1);
+  // Sums of c are those of one gate's rows each, whichever of the two gradients they are for.
+  p.k = mi::rn_bwd_plan(a->rows, a->D, a->dtype, p.gates > 1 && !p.own_rows && p.sum_c ? p.gates : 1);
   const size_t D = (size_t)a->D;
   p.part = (size_t)p.k.blocks * D * 4;
   p.dots = p.k.is_long && p.sum_c ? ((size_t)a->rows * 4 + 15) / 16 * 16 : 0;
@@ -181,6 +182,7 @@ int mi_residual_norm_backward(const mi_residual_norm_grad_args* a, void* workspa
   p.scale = a->scale;
   p.params_f32 = a->params_f32 != 0;
   p.gate_f32 = a->gate_f32 != 0;
+  p.own_gates = plan.own_rows;
   mi::rn_bwd_run(p, plan.k, a->dtype, a->stream_f32 != 0, s);
   const int lrc = launched("residual norm gradient");
   if (lrc != MI_OK || (!plan.sum_w && !plan.sum_c)) return lrc;
