@@ -21,16 +21,30 @@
 // 5.3 TB/s), small ones by a block's arithmetic: 32 quotients a lane and form.
 //
 // The quotient: t = x inv with inv = fp32(1 / scale), then t + (x - t scale)
-// inv in two fmas, which is x / scale correctly rounded (Markstein: inv is
-// correctly rounded, t within an ulp); a division's own sequence is 10
-// instructions.  Maxima are taken of the bits without their sign, which order
-// as the values do, with infinity and NaN above them.
+// inv in two fmas; a division's own sequence is 10 instructions.  t is within
+// 1.5 units of x / scale, so what the last fma rounds is within 2^-22 of one of
+// it, while a quotient of two fp32 numbers may be 2^-25 of one from halfway
+// between two others.  The rest was checked by enumeration.  A last place that
+// is off changes the 8-bit value only next to a border between two of them:
+// for every significand of the scale, every border and the 9 fp32 numbers
+// nearest to their product (1.2e9 pairs) the result is x / scale correctly
+// rounded.  Exponents do not matter as long as no bit of the residual x - t
+// scale falls below 2^-149.  Some do for scales under 2^-86 (e5m2; 2^-93 for
+// e4m3), and values beside borders came out as their neighbours: blocks with
+// scales below 2^-80 are divided with values and scale times 2^60 (but for the
+// least scale, with which, a power of two, t is exact), behind branches of the
+// wave (0.25 of 8.75 us for 1000 x 5000 with the transpose; values lifted in
+// place behind one branch took as long and more registers).
+//
+// Maxima are taken of the bits without their sign, which order as the values
+// do, with infinity and NaN above them.
 #pragma once
 #include "mi_norm.hpp"
 
 namespace mi {
 
 constexpr float kQuantMinScale = 0x1p-100f;
+constexpr float kQuantSmall = 0x1p-80f, kQuantLift = 0x1p60f;
 constexpr int kQuantThreads = 512;
 
 struct Quant {
@@ -70,6 +84,25 @@ __device__ __forceinline__ void scale_of(uint32_t most, bool e5m2, bool e8m0, fl
 __device__ __forceinline__ float quotient(float x, float scale, float inv) {
   const float t = x * inv;
   return __builtin_fmaf(__builtin_fmaf(-t, scale, x), inv, t);
+}
+// Whether a lane of the wave has such a small scale.  (fp16 values have none but
+// the least.)
+template <class T>
+__device__ __forceinline__ bool any_small(float scale) {
+  return !std::is_same<T, Fp16>::value && __builtin_amdgcn_ballot_w64(scale < kQuantSmall && scale > kQuantMinScale) != 0;
+}
+template <int N>
+__device__ __forceinline__ void divide(float (&t)[N], float scale, float inv, bool small) {
+  if (small) {
+    const bool own = scale < kQuantSmall;
+    const float up = own ? kQuantLift : 1.0f;
+    scale *= up;
+    inv *= own ? 1.0f / kQuantLift : 1.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) t[i] *= up;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) t[i] = quotient(t[i], scale, inv);
 }
 // Four values as bytes.
 __device__ __forceinline__ uint32_t fp8x4(float a, float b, float c, float d, bool e5m2) {
@@ -120,7 +153,7 @@ __device__ __forceinline__ void quantize_tile(const Quant& p, unsigned tile, boo
   __shared__ __attribute__((aligned(16))) uint8_t turned[TURNED ? 128 * 128 : 16];
   __shared__ __attribute__((aligned(16))) uint32_t most_of[TURNED || SQUARE ? WAVES : 1][128];
   __shared__ __attribute__((aligned(16))) float col_scale[TURNED && !SQUARE ? 128 : 4], col_inv[TURNED && !SQUARE ? 128 : 4];
-  __shared__ uint32_t half_most[2];
+  __shared__ uint32_t half_most[2];  // or whether 64 columns' scales have a small one
   const int tid = (int)threadIdx.x, wave = tid >> 6;
   const int group = tid >> 4, in_row = tid & 15;  // rows 4 group .. 4 group + 3, columns 8 in_row ..
   const int tiles_k = (p.K + 127) / 128;
@@ -193,6 +226,8 @@ __device__ __forceinline__ void quantize_tile(const Quant& p, unsigned tile, boo
         scale_of(most, p.e5m2, p.e8m0, scale, inv);
         col_scale[c] = scale;
         col_inv[c] = inv;
+        const bool small = any_small<T>(scale);
+        if ((tid & 63) == 0) half_most[tid >> 6] = small;
         if (tk * 128 + c < p.K) put_scale(p.scale_t, (size_t)tm * (size_t)p.K + tk * 128 + c, scale, p.e8m0);
       }
     }
@@ -211,6 +246,7 @@ __device__ __forceinline__ void quantize_tile(const Quant& p, unsigned tile, boo
   const bool edge_k = k + V > p.K;
   if (rows) {
     float scale[R], inv[R];
+    bool small;
     if constexpr (!SQUARE) {
       uint32_t most[R];
 #pragma unroll
@@ -228,6 +264,7 @@ __device__ __forceinline__ void quantize_tile(const Quant& p, unsigned tile, boo
       const uint32_t own = mine == 0 ? most[0] : mine == 1 ? most[1] : mine == 2 ? most[2] : most[3];
       float my_scale, my_inv;
       scale_of(own, p.e5m2, p.e8m0, my_scale, my_inv);
+      small = any_small<T>(my_scale);
       if (in_row < R && m0 + in_row < p.M) put_scale(p.scale, (size_t)tk * (size_t)p.M + m0 + in_row, my_scale, p.e8m0);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
@@ -235,6 +272,7 @@ __device__ __forceinline__ void quantize_tile(const Quant& p, unsigned tile, boo
         inv[r] = __shfl(my_inv, r, 16);
       }
     } else {
+      small = any_small<T>(all_scale);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         scale[r] = all_scale;
@@ -245,7 +283,8 @@ __device__ __forceinline__ void quantize_tile(const Quant& p, unsigned tile, boo
     for (int r = 0; r < R; ++r) {
       float t[V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) t[i] = quotient(to_f32(v[r].v[i]), scale[r], inv[r]);
+      for (int i = 0; i < V; ++i) t[i] = to_f32(v[r].v[i]);
+      divide(t, scale[r], inv[r], small);
       if (edge_k) {
 #pragma unroll
         for (int i = 0; i < V; ++i) t[i] = k + i < p.K ? t[i] : 0.0f;  // (a NaN scale leaves no zeros)
@@ -259,6 +298,8 @@ __device__ __forceinline__ void quantize_tile(const Quant& p, unsigned tile, boo
     const bool edge_m = m0 + R > p.M;
 #pragma unroll
     for (int r = 0; r < R; ++r) forget(v[r]);
+    const bool small = SQUARE ? any_small<T>(all_scale)
+                              : !std::is_same<T, Fp16>::value && __builtin_amdgcn_readfirstlane(half_most[0] | half_most[1]) != 0;
     f32x4_t scales = {}, invs = {};
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -271,7 +312,8 @@ __device__ __forceinline__ void quantize_tile(const Quant& p, unsigned tile, boo
       const float scale = SQUARE ? all_scale : scales[i % 4], inv = SQUARE ? all_inv : invs[i % 4];
       float t[R];
 #pragma unroll
-      for (int r = 0; r < R; ++r) t[r] = quotient(to_f32(v[r].v[i]), scale, inv);
+      for (int r = 0; r < R; ++r) t[r] = to_f32(v[r].v[i]);
+      divide(t, scale, inv, small);
       if (edge_m) {
 #pragma unroll
         for (int r = 0; r < R; ++r) t[r] = m0 + r < p.M ? t[r] : 0.0f;
