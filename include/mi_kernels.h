@@ -421,9 +421,12 @@ int mi_quantize_fp8(const mi_quantize_fp8_args* args, void* stream);
  * the matrix instructions drop of each 8 consecutive ones, below 2^-13 of the
  * largest (about 1e-5 of a result); one rounding.  Scales fp32, or exponents
  * (scale_e8m0), of any row and block strides in elements: lhs's one for each
- * row and block of 128, rhs's likewise or (rhs_square) one for 128 rows; the
- * product of two has to be finite.  Any M, N, K >= 0 (K = 0: a product of 0);
- * operands under 4 GiB, counting 256 rows past their end.  Rows that do not
+ * row and block of 128, rhs's likewise or (rhs_square) one for 128 rows.  The
+ * product of two fp32 ones is an fp32 number itself: it has to be finite, and
+ * below 2^-126 it is one of the multiples of 2^-149, so a block's share of the
+ * result is then off by up to 2^-150 of its unscaled sum (all of it, where the
+ * product is 2^-150 or less); powers of two have no such limit.  Any M, N, K >=
+ * 0 (K = 0: a product of 0); operands under 4 GiB, counting 256 rows past their end.  Rows that do not
  * start on 16 bytes are read from padded copies in the workspace.  cfg: one of
  * mi_fp8_config's, any split_k 1..16 that leaves no part empty, group_m (0:
  * 8); NULL: the library's choice. */

@@ -10,9 +10,11 @@
 // fp32 scales: each MFMA starts from 0, and its 4 results a lane are added to
 // the accumulators with one fma each, times ls rs, while the next MFMA runs:
 // 16 cycles of VALU work under 32 of the matrix core (32 with a scale for
-// each row of rhs, whose products with ls differ by column).  Powers of two
-// go to the MFMA itself, which scales each operand's 32 values as it reads
-// them and accumulates in place.
+// each row of rhs, whose products with ls differ by column).  ls rs is rounded
+// to fp32 before it meets a result, so below 2^-126 it loses digits; applied
+// one after the other the two would take 4 multiplications an MFMA more, and
+// overflow where ls alone is large.  Powers of two go to the MFMA itself, which
+// scales each operand's 32 values as it reads them and accumulates in place.
 //
 // The 8-bit MFMAs (all of them, the older 16x16x32 too) add 8 products at a
 // time, aligned to the largest, and drop what lies below 2^-13 of its binade;

@@ -138,7 +138,12 @@ def matmul_fp8(
     ``lhs``: e4m3 or e5m2, ``lhs_scale [M, ceil(K / 128)]``; ``rhs``: e4m3, ``rhs_scale [N, ceil(K / 128)]`` or, for 128
     rows at a time, ``[ceil(N / 128), ceil(K / 128)]``; both scales fp32 or both ``float8_e8m0fnu``, of any strides (those
     of ``quantize_fp8`` are read fastest); ``out``: bf16.  ``cfg``: one of ``fp8_configs()``, any
-    ``split_k`` and ``group_m``; None for the library's choice."""
+    ``split_k`` and ``group_m``; None for the library's choice.
+
+    The values' products are exact.  The matrix instructions add 8 consecutive ones at a time and drop what lies below
+    2^-13 of the largest (about 1e-5 of a result of normally distributed values, where the rounding to bf16 is up to 2^-8);
+    these sums are added in fp32.  The product of two fp32 scales is rounded to fp32 too: it has to be finite, and below
+    2^-126 it is a multiple of 2^-149."""
     if cfg is None:
         done = _torch_call.matmul_fp8(lhs, lhs_scale, rhs, rhs_scale, out)
         if done is not None:
