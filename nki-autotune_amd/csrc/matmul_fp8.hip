@@ -405,9 +405,9 @@ int check_quant(long long M, long long K) {
 }
 // Whether a matrix's two forms are taken by a block each: few tiles, whose time
 // is that of a block's arithmetic and not of reading the values (both forms,
-// bf16, 300 x 700 6.0 us and 4.5, 1000 x 5000 9.0 and 7.6, 4096 x 2560 12.1 and
-// 10.7, 4096 x 4096 16.9 and 18.1; fp32 1000 x 1501 6.1 and 4.9, 2048 x 4096
-// 11.2 and 11.4).
+// bf16, in graphs, 300 x 700 6.5 us and 4.7, 1000 x 5000 9.2 and 7.8, 4096 x 2560
+// 12.5 and 11.3, 4096 x 4096 17.6 and 18.2; fp32 1000 x 1501 6.4 and 5.0, 2048 x
+// 4096 11.4 and 11.4).
 bool in_halves(const Quant& p, bool light) {
   return p.q && p.q_t && blocks128(p.M) * blocks128(p.K) <= (light ? 3 : 1) * mi::capi::device_cus();
 }

@@ -4,11 +4,14 @@
 #include "mi_mm_fp8.hpp"
 
 // block_m, block_n, waves, lds_stages, rhs read non-temporally; then what the
-// library's choice goes by: in microseconds a K tile of a block alone on its
-// compute unit with scales for 128 rows of rhs, for each row, and with powers
-// of two, a K tile of one of several that share the unit, a block's beginning
-// and end; how many of its blocks a unit holds; and TB/s of all of them
-// together where rhs comes from HBM.
+// library's choice goes by, terms of an estimate in microseconds: a K tile of a
+// block alone on its compute unit with scales for 128 rows of rhs, for each row,
+// and with powers of two, a K tile of one of several that share the unit, a
+// block's beginning and end; how many of its blocks a unit holds; and TB/s of
+// all of them together where rhs comes from HBM.  Of the two kinds of K tiles
+// the one that makes the longer time counts.  Where one block fills a unit that
+// is the larger of two terms, and the other is where the fit began, 0.350, which
+// says nothing of a K tile.
 //
 // Fitted (least squares of the logarithm, near the fastest config of each
 // shape) to all of them with up to 16 parts, timed in graphs at 42 shapes from

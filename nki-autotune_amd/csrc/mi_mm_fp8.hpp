@@ -33,10 +33,12 @@
 // (the memory behind a row may hold anything).
 //
 // 8192^3 with fp32 scales 437-460 us by box (2.4-2.5 PFLOP/s; the library's
-// product with one scale for all of a matrix 334-357), with powers of two 396.
-// Bound by the chip's power: a few 256 x 256 blocks alone run at 2.4 GHz and
-// take 1.21 us a K tile (1.12 with powers of two; its MFMAs 0.85), all of them
-// run at 1.88 GHz and take 1.7, with the matrix cores busy 62 % of the cycles.
+// product with one scale for all of a matrix 334-357), 502-514 with one for each
+// row of rhs, whose 8 VALU instructions an MFMA take as long as it, with powers of
+// two 396.  A few 256 x 256 blocks alone run at 2.4 GHz and take 1.21 us a K
+// tile (1.12 with powers of two), of which its MFMAs are 0.85; all of them run
+// at 1.88 GHz, the chip's power limit, and take 1.7, 1.40 times as long where
+// the clock is 1.28 times lower, with the matrix cores busy 62 % of the cycles.
 // So blocks that follow one another without a pause, the next one's loads
 // behind the last MFMAs, were no faster (441 us and 438).  16 x 28672 x 8192
 // reads the weight at 5.6 TB/s, 42 us.

@@ -13,8 +13,8 @@
 // the lanes and the 8 waves) or the block's.  q is written 8 bytes a lane; the
 // transpose's bytes are turned in LDS, where a lane writes the 4 rows of a
 // column at once, and written 16 bytes a lane.  (8 rows a lane of 256 threads:
-// 1000 x 5000 with the transpose 12.7 us, so 9.0, 7.6 with a block for each of
-// the two forms.)  Scales of 1 x 128 blocks lie with the rows consecutive, as
+// 1000 x 5000 with the transpose 12.7 us, so 9.2, 7.8 with a block for each of
+// the two forms, in graphs; calls one after the other 8.7.)  Scales of 1 x 128 blocks lie with the rows consecutive, as
 // the workgroup has them.
 //
 // Large matrices are bound by HBM (28672 x 8192 fp32 with the transpose 264 us,
@@ -33,8 +33,10 @@
 // e4m3), and values beside borders came out as their neighbours: blocks with
 // scales below 2^-80 are divided with values and scale times 2^60 (but for the
 // least scale, with which, a power of two, t is exact), behind branches of the
-// wave (0.25 of 8.75 us for 1000 x 5000 with the transpose; values lifted in
-// place behind one branch took as long and more registers).
+// wave, which cost 0.25 of 8.75 us for 1000 x 5000 bf16 with the transpose and
+// 0.8 of 18.4 for 4096 x 4096.  (Values lifted in place behind one branch, or
+// all quotients twice in the code behind one: as long for the first, 0.3 less
+// for the second.)
 //
 // Maxima are taken of the bits without their sign, which order as the values
 // do, with infinity and NaN above them.

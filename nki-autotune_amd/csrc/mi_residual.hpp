@@ -30,8 +30,14 @@
 //
 // Bound by HBM: 16384 x 8192 bf16 with both norms 207 us (5.2 TB/s; a copy
 // reaches 5.0), the gradients of 16384 x 4096 with an fp32 stream 218 us (5.6
-// TB/s with the column sums' second launch, 5 us).  Few rows are bound by the
-// launches: 8 x 4096 3.9 us of a kernel, 1000 x 1501 fp32 gradients 11.5 + 5.4.
+// TB/s with the column sums' second launch, 5 us).  A gate for each row: 16384 x
+// 8192 bf16 266 us forward (5.0 TB/s) and 364 back (5.9).  Few rows are bound by
+// the launches: 8 x 4096 3.9 us of a kernel, 1000 x 1501 fp32 gradients 11.5 +
+// 5.4.  Rows past 8192 wait for their own loads (8192 x 16384 bf16 with both
+// norms 237 us, 4.5 TB/s), and longer ones, past 8192 in the gradients, are read
+// two or three times, from the caches at best: 4096 x 32768 247 us without a
+// norm after the block and 350 with, the gradients of 8192 x 16384 655 (2.5 TB/s
+// of what has to move), their column sums' kernel among them.
 #pragma once
 #include "mi_norm.hpp"
 
@@ -294,7 +300,7 @@ __global__ __launch_bounds__(L* GROUPS) void residual_norm_bwd_kernel(const RnBw
   Pack<T> ny[G], nx[G];
   Pack<R, V> nd[G], nh[G];
   float nrstd, npost = 1.0f;
-  // (What is not there is read as the rows of hidden, which is, and left out.)
+  // (What is not there is read as rows that are, x as dy and dhidden as hidden, and left out.)
   const T* xp = p.x ? (const T*)p.x : (const T*)p.dy;
   const size_t ldx = p.x ? (size_t)p.ldx : (size_t)p.lddy;
   const R* dhp = p.dhidden ? (const R*)p.dhidden : (const R*)p.hidden;

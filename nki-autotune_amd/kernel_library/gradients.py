@@ -72,7 +72,7 @@ def clip_grad_norm(
 
     ``out``: where the clipped gradients go, of their gradients' types and shapes: ``grads`` itself for in place, or
     tensors apart from them; None for new ones.  An infinite norm clips to 0 (and its infinities to NaN), a NaN one to
-    NaN."""
+    NaN, as does an infinite one where ``max_norm`` is infinite too."""
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must be >= 0, got {max_norm}")
     if not 0.0 <= eps < 3e38:
